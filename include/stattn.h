@@ -262,6 +262,65 @@ int stattn_broadcast_params(stattn_handle* h, int root);
 /* SUM `n` host floats over the ranks in place (reported cost, counters); n <= 64 */
 int stattn_allreduce_scalars(stattn_handle* h, float* vals, int n);
 
+/* ---- operators on device memory: 4-bit matrices and drafted words ------------------------------------
+ * The pieces of drafted sampling (stattn_sample_drafted) as operators of their own, on the caller's device buffers: no handle, no host
+ * copies.  Every pointer ending in `_dev` is memory of GPU `device`; the work is enqueued on `stream` (a hipStream_t of that GPU, or
+ * NULL: its default stream) and the call returns; nothing is allocated, so calls may be captured into a hipGraph, and calls on
+ * different streams are independent of each other as long as they share no output and no workspace.  The current device of the calling
+ * thread is left as it was.  Return value as everywhere (0 or a STATTN_E* code); the message of the calling thread's last failed
+ * operator is stattn_op_error().
+ *
+ * The 4-bit form (OCP microscaling, MXFP4) of a (rows, cols) matrix: kp = cols rounded up to a multiple of 128;
+ *   codes  (rows, kp / 2) bytes, two columns a byte, the even one in the low half: sign, 2 bits of exponent, 1 of mantissa
+ *          (0, 0.5, 1, 1.5, 2, 3, 4, 6);
+ *   scales (rows, kp / 32) bytes: byte s of a block of 32 columns multiplies its codes by 2^(s - 127); 255 makes the block NaN.
+ * Both 16-byte aligned.  Columns behind the last one hold code 0 (they must, when the form comes from elsewhere and is multiplied). */
+#define STATTN_F32 0
+#define STATTN_BF16 1
+#define STATTN_F16 2
+const char* stattn_op_error(void);
+
+/* Element (r, c) of the matrix is x_dev[r * row_stride + c * col_stride], of type `dtype`; blocks run along c.  A matrix stored the other
+ * way round (ff_logit_W is (dim_word, n_words); its 4-bit form has a row per word) is passed with row_stride = 1.  The scale of a block
+ * whose largest magnitude is a: 2^(floor(log2 a) - 2), not under 2^-126 (a block of zeros: 1); values are rounded to the nearest code,
+ * ties to the even code, and to 6 beyond 6.  A block with an infinity or NaN becomes NaN. */
+int stattn_mx4_quantize(int device, void* stream, const void* x_dev, int dtype, int64_t rows, int64_t cols,
+                        int64_t row_stride, int64_t col_stride, void* codes_dev, void* scales_dev);
+/* out (rows, cols), row stride ld_out, of type `dtype`: the numbers the form stands for, rounded to the type */
+int stattn_mx4_dequantize(int device, void* stream, const void* codes_dev, const void* scales_dev, int64_t rows, int64_t cols,
+                          void* out_dev, int dtype, int64_t ld_out);
+/* y[i][j] = sum_c a[i][c] w[j][c] + bias[j]: a (m, k) and w (n, k) in the 4-bit form, bias float32 or NULL, y (m, n) of type `dtype`
+ * with row stride ld_y.  Products are exact, sums are in fp32, rounded once to the type. */
+int stattn_mx4_matmul(int device, void* stream, const void* a_codes_dev, const void* a_scales_dev, const void* w_codes_dev,
+                      const void* w_scales_dev, int64_t m, int64_t n, int64_t k, const float* bias_dev,
+                      void* y_dev, int dtype, int64_t ld_y);
+/* The same with a = x (m, k) of type `dtype`, row stride ld_x, brought into the 4-bit form on the way: the result is that of
+ * stattn_mx4_quantize followed by stattn_mx4_matmul.  y is of x's type.  `workspace_dev`: stattn_mx4_linear_workspace(m, n, k) bytes,
+ * 16-byte aligned, overwritten (may be NULL when that is 0); not to be shared by calls that can run at the same time. */
+size_t stattn_mx4_linear_workspace(int64_t m, int64_t n, int64_t k);
+int stattn_mx4_linear(int device, void* stream, const void* x_dev, int dtype, int64_t ld_x, const void* w_codes_dev,
+                      const void* w_scales_dev, int64_t m, int64_t n, int64_t k, const float* bias_dev, void* y_dev, int64_t ld_y,
+                      void* workspace_dev, size_t workspace_bytes);
+
+/* Drafted words of b captions checked against the decoder's own distribution.  draft (b, j) word indices, the first lens[i] of row i
+ * count (lens NULL: all j; values outside [0, j] are taken as the nearer end); target (b, j + 1, v): the decoder's next-word
+ * probabilities in front of each drafted word and behind the last; proposal (b, j, v): the distributions the words were drawn from, or
+ * NULL when each was certain (arg-max drafts).  Both of type `dtype`, v contiguous, strides in elements.  accept_u (b, j), draw_u (b):
+ * uniform numbers in [0, 1).
+ * Word d at position p is kept while accept_u * proposal[p][d] < target[p][d]; behind the kept words one word is drawn by draw_u: the
+ * first whose running sum of weights exceeds draw_u * total, weights max(target - proposal, 0) at the refused position (target itself
+ * if all of them are 0), or target behind a draft that was kept whole.  accepted[i] = kept words; words row i = the kept words, the
+ * drawn one, -1 from there on.  The captions that result are samples of the target's distribution.  Products and sums are in 64 bits;
+ * weights that are NaN count as 0; a drafted word outside [0, v) is refused; a row without any weight draws -1.
+ * `workspace_dev`: stattn_verify_draft_workspace(b, j, v) bytes, 16-byte aligned, overwritten; not to be shared by calls that can run
+ * at the same time. */
+size_t stattn_verify_draft_workspace(int64_t b, int64_t j, int64_t v);
+int stattn_verify_draft(int device, void* stream, const int64_t* draft_dev, int64_t draft_ld, const void* target_dev,
+                        int64_t target_stride_b, int64_t target_stride_j, const void* proposal_dev, int64_t proposal_stride_b,
+                        int64_t proposal_stride_j, int dtype, const float* accept_u_dev, int64_t accept_ld, const float* draw_u_dev,
+                        const int32_t* lens_dev, int64_t b, int64_t j, int64_t v, int64_t* words_dev, int64_t words_ld,
+                        int32_t* accepted_dev, void* workspace_dev, size_t workspace_bytes);
+
 /* ---- measurement hooks (bench.py's per-kernel rooflines) -------------------------------------------- */
 /* Average duration (ms) of the named kernel class over the last stattn_forward_train (or the stattn_beam_search /
  * f_next calls since profiling was switched on; a profiled beam search launches its words eagerly instead of replaying

@@ -31,6 +31,8 @@ class _Options(C.Structure):
 _F = C.POINTER(C.c_float)
 _I64 = C.POINTER(C.c_int64)
 _H = C.c_void_p
+_P = C.c_void_p         # device memory or a stream
+_I = C.c_int64
 
 _SIGNATURES = {
     # name: (restype, argtypes)
@@ -81,6 +83,14 @@ _SIGNATURES = {
     "stattn_allreduce_scalars": (C.c_int, [_H, _F, C.c_int]),
     "stattn_comm_stats": (C.c_int, [_H, C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int), _F]),
     "stattn_comm_library_path": (C.c_char_p, []),
+    "stattn_op_error": (C.c_char_p, []),
+    "stattn_mx4_quantize": (C.c_int, [C.c_int, _P, _P, C.c_int, _I, _I, _I, _I, _P, _P]),
+    "stattn_mx4_dequantize": (C.c_int, [C.c_int, _P, _P, _P, _I, _I, _P, C.c_int, _I]),
+    "stattn_mx4_matmul": (C.c_int, [C.c_int, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, C.c_int, _I]),
+    "stattn_mx4_linear_workspace": (C.c_size_t, [_I, _I, _I]),
+    "stattn_mx4_linear": (C.c_int, [C.c_int, _P, _P, C.c_int, _I, _P, _P, _I, _I, _I, _P, _P, _I, _P, C.c_size_t]),
+    "stattn_verify_draft_workspace": (C.c_size_t, [_I, _I, _I]),
+    "stattn_verify_draft": (C.c_int, [C.c_int, _P, _P, _I, _P, _I, _I, _P, _I, _I, C.c_int, _P, _I, _P, _P, _I, _I, _I, _P, _I, _P, _P, C.c_size_t]),
     "stattn_set_profiling": (C.c_int, [_H, C.c_int]),
     "stattn_get_kernel_ms": (C.c_int, [_H, C.c_int, _F, C.POINTER(C.c_int)]),
 }

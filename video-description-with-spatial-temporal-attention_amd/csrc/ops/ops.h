@@ -1,0 +1,43 @@
+// Launchers of the device-memory operators (csrc/api_ops.cpp checks the arguments, these trust them).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace stattn {
+
+enum OpType { OP_F32 = 0, OP_BF16 = 1, OP_F16 = 2 };
+
+// The 4-bit form of a (rows, cols) matrix: codes [rows][kp / 2] bytes (even column in the low half), scales [rows][kp / 32] bytes,
+// kp = cols rounded up to 128.  Both pointers 16-byte aligned.
+struct Mx4View { const uint8_t* codes; const uint8_t* scales; int64_t rows; int64_t cols; };
+inline int64_t mx4_kp(int64_t cols) { return (cols + 127) / 128 * 128; }
+
+struct Mx4QuantArgs {
+    const void* x; OpType type; int64_t rows, cols, row_stride, col_stride;      // element (r, c) at x[r * row_stride + c * col_stride]
+    uint8_t* codes; uint8_t* scales;
+};
+hipError_t launch_mx4_quantize(hipStream_t s, const Mx4QuantArgs& a);
+hipError_t launch_mx4_dequantize(hipStream_t s, const Mx4View& q, void* out, OpType type, int64_t ld);
+
+struct Mx4GemmArgs {
+    Mx4View a, w;                        // y[m][n] = sum_k a[m][k] w[n][k] + bias[n]
+    const float* bias;                   // or null
+    void* y; OpType type; int64_t ldy;
+};
+hipError_t launch_mx4_matmul(hipStream_t s, const Mx4GemmArgs& g);
+
+struct VerifyArgs {
+    const int64_t* draft; int64_t draft_ld;
+    const void* target; int64_t target_b, target_j;          // strides of the caption and of the position, in elements
+    const void* proposal; int64_t proposal_b, proposal_j;    // or null: every drafted word was certain
+    OpType type;
+    const float* accept_u; int64_t accept_ld;
+    const float* draw_u;
+    const int32_t* lens;                                     // or null: every draft has j words
+    int64_t b; int j; int64_t v;
+    int64_t* words; int64_t words_ld; int32_t* accepted;
+};
+hipError_t launch_verify_draft(hipStream_t s, const VerifyArgs& a);
+
+}  // namespace stattn
