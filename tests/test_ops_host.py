@@ -50,6 +50,7 @@ def test_dequantize_refusals():
 def test_matmul_and_linear_refusals():
     f = lib().stattn_mx4_matmul
     refused(f(0, None, A, A, A, A, 4, 8, 32, None, A, 0, 7), "ld_y")
+    refused(f(0, None, A, A, A, A, 4, 8, 32, None, A, 0, 1 << 22), "ld_y")
     refused(f(0, None, A, A, A, A, 4, 8, 32, None, A, 9, 8), "dtype")
     refused(f(0, None, A, A, A, A, 4, 8, 32, None, None, 0, 8), "null y")
     refused(f(0, None, A, A, A, A + 4, 4, 8, 32, None, A, 0, 8), "aligned")
@@ -71,8 +72,8 @@ def test_matmul_and_linear_refusals():
 def test_verify_refusals():
     f = lib().stattn_verify_draft
 
-    def call(b=2, j=3, v=10, dtype=0, draft=A, target=A, proposal=A, au=A, du=A, words=A, ld=4, acc=A, ws=A, nws=1 << 30):
-        return f(0, None, draft, j, target, (j + 1) * v, v, proposal, j * v, v, dtype, au, j, du, None, b, j, v, words, ld, acc, ws, nws)
+    def call(b=2, j=3, v=10, dtype=0, draft=A, target=A, proposal=A, au=A, du=A, words=A, ld=4, acc=A):
+        return f(0, None, draft, j, target, (j + 1) * v, v, proposal, j * v, v, dtype, au, j, du, None, b, j, v, words, ld, acc)
     refused(call(dtype=5), "dtype")
     refused(call(v=0), "v = 0")
     refused(call(j=-1), "j = -1")
@@ -81,11 +82,6 @@ def test_verify_refusals():
     refused(call(ld=3), "words_ld")
     for name in ("draft", "target", "au", "du", "words", "acc"):
         refused(call(**{name: None}), "null")
-    need = lib().stattn_verify_draft_workspace(2, 3, 200000)
-    if need:
-        refused(call(v=200000, nws=need - 1), "workspace")
-        refused(call(v=200000, ws=None), "workspace")
-        refused(call(v=200000, ws=A + 4), "workspace")
     assert call(b=0) == 0
 
 

@@ -1,73 +1,125 @@
-// Writing matrices in microscaled 4 bits and reading them back.
+// Writing matrices in microscaled 4 bits and reading them back.  Both are bound by memory: 4 (2) bytes an element on one side, 17 / 32 on
+// the other.
 #include "mx4_inl.h"
 
 namespace stattn {
 
-// One thread per block of 32 columns.
-template <OpType T>
-__global__ __launch_bounds__(256) void mx4_quantize_kernel(Mx4QuantArgs a, int64_t kb, int64_t nblk) {
+// x row-major.  A lane takes eight columns (one or two 16-byte loads) and writes the word of their codes, so a wave reads and writes
+// whole lines; the four lanes of a block find its scale by two moves inside the quad.  (A lane per block, 32 columns each, read lines in
+// eight or four pieces: the regions of a batch, 13312 x 4096 bf16, took 125 us instead of XX.)
+template <OpType T, bool WIDE>
+__global__ __launch_bounds__(256) void mx4_quantize_rows_kernel(Mx4QuantArgs a, unsigned words, int64_t n) {
     typedef typename Elem<T>::type E;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= nblk) return;
-    const int64_t r = i / kb, b = i % kb;
-    const E* x = static_cast<const E*>(a.x) + r * a.row_stride;
-    float v[32];
-    unsigned top = 0;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        const int64_t c = b * 32 + j;
-        v[j] = c < a.cols ? (float)x[c * a.col_stride] : 0.f;
-        top = max(top, abs_bits(v[j]));
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {      // n and the steps are multiples of 4
+        const int64_t r = n >> 32 ? i / words : (int64_t)((unsigned)i / words);
+        const int c = (int)(i - r * words) * 8, here = (int)max(min(a.cols - c, (int64_t)8), (int64_t)0);
+        Eight<T, WIDE> x;
+        float v[8];
+        x.take(static_cast<const E*>(a.x) + r * a.row_stride, c, here);
+        x.put(v, here);
+        const unsigned byte = mx4_scale_byte(quad_max(top8(v)));
+        reinterpret_cast<unsigned*>(a.codes)[i] = mx4_codes8(v, byte);
+        if ((threadIdx.x & 3) == 0) a.scales[i >> 2] = (uint8_t)byte;
     }
-    const unsigned byte = mx4_scale_byte(top);
-    uint4 o;
-    o.x = mx4_codes8(v, byte); o.y = mx4_codes8(v + 8, byte); o.z = mx4_codes8(v + 16, byte); o.w = mx4_codes8(v + 24, byte);
-    *reinterpret_cast<uint4*>(a.codes + i * 16) = o;
-    a.scales[i] = (uint8_t)byte;
+}
+
+// x column-major (the rows of the form are neighbours in memory), and any other pair of strides.  A workgroup takes 64 rows x 128 columns
+// of the form: a lane reads the 32 values of a block down its row, 64 lanes side by side; the 16-byte blocks meet in LDS, from where each
+// row's 64 bytes leave together.
+template <OpType T>
+__global__ __launch_bounds__(256) void mx4_quantize_cols_kernel(Mx4QuantArgs a, unsigned row_tiles, unsigned kp128) {
+    typedef typename Elem<T>::type E;
+    __shared__ uint4 code[64][5];                    // a row's four blocks, one slot apart from the next row's banks
+    __shared__ uint8_t scale[64][4];
+    const int lane = threadIdx.x & 63, blk = threadIdx.x >> 6;
+    for (int64_t t = blockIdx.x; t < (int64_t)row_tiles * kp128; t += gridDim.x) {
+        const int64_t r0 = t % row_tiles * 64, c0 = t / row_tiles * 128, r = r0 + lane, c = c0 + blk * 32;
+        float v[32];
+        const E* x = static_cast<const E*>(a.x) + r * a.row_stride + c * a.col_stride;
+        const int here = r < a.rows ? (int)max(min(a.cols - c, (int64_t)32), (int64_t)0) : 0;
+        if (here == 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = (float)x[j * a.col_stride];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = j < here ? (float)x[j * a.col_stride] : 0.f;
+        }
+        const unsigned byte = mx4_scale_byte(max(max(top8(v), top8(v + 8)), max(top8(v + 16), top8(v + 24))));
+        code[lane][blk] = make_uint4(mx4_codes8(v, byte), mx4_codes8(v + 8, byte), mx4_codes8(v + 16, byte), mx4_codes8(v + 24, byte));
+        scale[lane][blk] = (uint8_t)byte;
+        __syncthreads();
+        const int64_t ro = r0 + (threadIdx.x >> 2);
+        if (ro < a.rows) {
+            const int64_t at = ro * kp128 * 4 + c0 / 32;
+            reinterpret_cast<uint4*>(a.codes)[at + (threadIdx.x & 3)] = code[threadIdx.x >> 2][threadIdx.x & 3];
+            if ((threadIdx.x & 3) == 0) *reinterpret_cast<unsigned*>(a.scales + at) = *reinterpret_cast<const unsigned*>(scale[threadIdx.x >> 2]);
+        }
+        __syncthreads();
+    }
+}
+
+constexpr int64_t FULL = 256 * 16;      // workgroups that keep the chip busy; more elements are walked by the same ones
+
+template <OpType T>
+static hipError_t quantize(hipStream_t s, const Mx4QuantArgs& a) {
+    const int64_t kp = mx4_kp(a.cols);
+    if (a.col_stride == 1 || a.cols == 1) {
+        const int64_t n = a.rows * (kp / 8);
+        const bool wide = eights_are_wide(a.x, a.row_stride, a.cols, sizeof(typename Elem<T>::type));
+        const dim3 grid((unsigned)std::min((n + 255) / 256, FULL));
+        if (wide) mx4_quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(a, (unsigned)(kp / 8), n);
+        else mx4_quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(a, (unsigned)(kp / 8), n);
+    } else {
+        const int64_t rt = (a.rows + 63) / 64;
+        mx4_quantize_cols_kernel<T><<<dim3((unsigned)std::min(rt * (kp / 128), FULL)), 256, 0, s>>>(a, (unsigned)rt, (unsigned)(kp / 128));
+    }
+    return hipGetLastError();
 }
 
 hipError_t launch_mx4_quantize(hipStream_t s, const Mx4QuantArgs& a) {
-    const int64_t kb = mx4_kp(a.cols) / 32, n = a.rows * kb;
-    const dim3 grid((unsigned)((n + 255) / 256));
-    switch (a.type) {
-        case OP_F32: mx4_quantize_kernel<OP_F32><<<grid, 256, 0, s>>>(a, kb, n); break;
-        case OP_BF16: mx4_quantize_kernel<OP_BF16><<<grid, 256, 0, s>>>(a, kb, n); break;
-        case OP_F16: mx4_quantize_kernel<OP_F16><<<grid, 256, 0, s>>>(a, kb, n); break;
-    }
-    return hipGetLastError();
+    return a.type == OP_F32 ? quantize<OP_F32>(s, a) : a.type == OP_BF16 ? quantize<OP_BF16>(s, a) : quantize<OP_F16>(s, a);
 }
 
-// One thread per eight columns: a word of codes, the block's scale, eight values.  The code is turned into its number first and
+// A lane per eight columns: a word of codes, the block's scale, one or two 16-byte stores.  The code is turned into its number first and
 // multiplied by the scale after, so that the smallest scales (2^-127 is subnormal) and NaN need no case of their own.
 template <OpType T>
-__global__ __launch_bounds__(256) void mx4_dequantize_kernel(Mx4View q, typename Elem<T>::type* out, int64_t ld, int64_t w8, int64_t n) {
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(Mx4View q, typename Elem<T>::type* out, int64_t ld, unsigned words, int64_t n, bool wide) {
     typedef typename Elem<T>::type E;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const int64_t r = i / w8, c = i % w8;
-    const unsigned w = reinterpret_cast<const unsigned*>(q.codes)[i];
-    const float s = mx4_scale(q.scales[i >> 2]);
-    float v[8];
-    auto put = [&](int at, auto two) { v[at] = two[0] * s; v[at + 1] = two[1] * s; };
-    put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0));
-    put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1));
-    put(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2));
-    put(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3));
-    E* o = out + r * ld + c * 8;
+    typedef E e8 __attribute__((ext_vector_type(8)));
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = n >> 32 ? i / words : (int64_t)((unsigned)i / words);
+        const int c = (int)(i - r * words) * 8;
+        if (c >= q.cols) continue;
+        const unsigned w = reinterpret_cast<const unsigned*>(q.codes)[i];
+        const float s = mx4_scale(q.scales[i >> 2]);
+        e8 v;
+        auto put = [&](int at, auto two) { v[at] = (E)(two[0] * s); v[at + 1] = (E)(two[1] * s); };
+        put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0));
+        put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1));
+        put(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2));
+        put(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3));
+        E* o = out + r * ld + c;
+        if (wide && c + 8 <= q.cols) {
+            *reinterpret_cast<e8*>(o) = v;
+        } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (c * 8 + j < q.cols) o[j] = (E)v[j];
+            for (int j = 0; j < 8; ++j)
+                if (c + j < q.cols) o[j] = v[j];
+        }
+    }
+}
+
+template <OpType T>
+static hipError_t dequantize(hipStream_t s, const Mx4View& q, void* out, int64_t ld) {
+    typedef typename Elem<T>::type E;
+    const int64_t words = mx4_kp(q.cols) / 8, n = q.rows * words;
+    const bool wide = (reinterpret_cast<uintptr_t>(out) & (sizeof(E) * 8 - 1)) == 0 && ld % 8 == 0;
+    mx4_dequantize_kernel<T><<<dim3((unsigned)std::min((n + 255) / 256, FULL)), 256, 0, s>>>(q, static_cast<E*>(out), ld, (unsigned)words, n, wide);
+    return hipGetLastError();
 }
 
 hipError_t launch_mx4_dequantize(hipStream_t s, const Mx4View& q, void* out, OpType type, int64_t ld) {
-    const int64_t w8 = mx4_kp(q.cols) / 8, n = q.rows * w8;
-    const dim3 grid((unsigned)((n + 255) / 256));
-    switch (type) {
-        case OP_F32: mx4_dequantize_kernel<OP_F32><<<grid, 256, 0, s>>>(q, static_cast<float*>(out), ld, w8, n); break;
-        case OP_BF16: mx4_dequantize_kernel<OP_BF16><<<grid, 256, 0, s>>>(q, static_cast<__bf16*>(out), ld, w8, n); break;
-        case OP_F16: mx4_dequantize_kernel<OP_F16><<<grid, 256, 0, s>>>(q, static_cast<_Float16*>(out), ld, w8, n); break;
-    }
-    return hipGetLastError();
+    return type == OP_F32 ? dequantize<OP_F32>(s, q, out, ld) : type == OP_BF16 ? dequantize<OP_BF16>(s, q, out, ld) : dequantize<OP_F16>(s, q, out, ld);
 }
 
 }  // namespace stattn

@@ -8,6 +8,7 @@
 
 namespace stattn {
 
+typedef int i32x4v __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef float f32x16v __attribute__((ext_vector_type(16)));
@@ -37,6 +38,44 @@ __device__ __forceinline__ unsigned mx4_codes8(const float* v, unsigned byte) {
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], s, 3);
     return byte == 255u ? 0u : c;
 }
+// the largest of four neighbouring lanes (a quad), in each of them
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));     // quad_perm [1, 0, 3, 2]
+    return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));  // quad_perm [2, 3, 0, 1]
+}
+__device__ __forceinline__ unsigned top8(const float* v) {
+    unsigned t = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t = max(t, abs_bits(v[j]));
+    return t;
+}
+// Eight neighbouring elements as they lie in memory: `take` requests them and `put` turns them into floats, so that a caller can have
+// several requests on their way.  Elements from number n (0 .. 8) on are not there and become 0.  WIDE: x is 16-byte aligned and n is
+// 0 or 8, one or two 16-byte loads without a branch (from the row's start where nothing is there); else element by element.
+template <OpType T, bool WIDE>
+struct Eight {
+    typedef typename Elem<T>::type E;
+    typedef E vec __attribute__((ext_vector_type(16 / sizeof(E))));
+    vec raw[WIDE ? sizeof(E) / 2 : 1];
+    E one[WIDE ? 1 : 8];
+    __device__ __forceinline__ void take(const E* row, int64_t c, int n) {
+        if constexpr (WIDE) {
+            const vec* x = reinterpret_cast<const vec*>(row + (n > 0 ? c : 0));
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(E) / 2; ++j) raw[j] = x[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) one[j] = row[j < n ? c + j : 0];
+        }
+    }
+    __device__ __forceinline__ void put(float* v, int n) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (WIDE) v[j] = n > 0 ? (float)raw[j / (16 / sizeof(E))][j % (16 / sizeof(E))] : 0.f;
+            else v[j] = j < n ? (float)one[j] : 0.f;
+        }
+    }
+};
 // the fp32 value of a scale byte (0 is 2^-127, a subnormal; 255 is NaN)
 __device__ __forceinline__ float mx4_scale(unsigned byte) {
     return __builtin_bit_cast(float, byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23);

@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 namespace stattn {
@@ -11,7 +12,12 @@ enum OpType { OP_F32 = 0, OP_BF16 = 1, OP_F16 = 2 };
 // The 4-bit form of a (rows, cols) matrix: codes [rows][kp / 2] bytes (even column in the low half), scales [rows][kp / 32] bytes,
 // kp = cols rounded up to 128.  Both pointers 16-byte aligned.
 struct Mx4View { const uint8_t* codes; const uint8_t* scales; int64_t rows; int64_t cols; };
-inline int64_t mx4_kp(int64_t cols) { return (cols + 127) / 128 * 128; }
+__host__ __device__ inline int64_t mx4_kp(int64_t cols) { return (cols + 127) / 128 * 128; }
+
+// whether every eight columns of a row-major matrix are one or two aligned 16-byte loads
+inline bool eights_are_wide(const void* x, int64_t ld, int64_t cols, size_t size) {
+    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * (int64_t)size % 16 == 0 && cols % 8 == 0;
+}
 
 struct Mx4QuantArgs {
     const void* x; OpType type; int64_t rows, cols, row_stride, col_stride;      // element (r, c) at x[r * row_stride + c * col_stride]
@@ -26,6 +32,16 @@ struct Mx4GemmArgs {
     void* y; OpType type; int64_t ldy;
 };
 hipError_t launch_mx4_matmul(hipStream_t s, const Mx4GemmArgs& g);
+
+// The same with x (m, k) of `type`, brought into the 4-bit form inside the launch: for few rows, where one launch and no trip of x's 4-bit
+// form through memory are what counts (api_ops.cpp has the rule).
+struct Mx4LinearArgs {
+    const void* x; OpType type; int64_t m, ldx;
+    Mx4View w;
+    const float* bias;
+    void* y; int64_t ldy;
+};
+hipError_t launch_mx4_linear_few(hipStream_t s, const Mx4LinearArgs& a);
 
 struct VerifyArgs {
     const int64_t* draft; int64_t draft_ld;

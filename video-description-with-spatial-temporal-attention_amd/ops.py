@@ -17,6 +17,10 @@ except ImportError:
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+_U8, _F32, _I32, _I64 = torch.uint8, torch.float32, torch.int32, torch.int64
+_empty = torch.empty
+# The checks below are written out, plain comparisons on the way of a good call: of the 7 us that a small product takes a caller, 3.5 are
+# the launch and 1.7 the result's allocation.
 
 
 def _fail(rc):
@@ -24,20 +28,17 @@ def _fail(rc):
     raise ValueError(msg) if rc == -1 else _native.NativeError("libstattn error %d: %s" % (rc, msg))
 
 
-def _float(t, name):
-    if t.dtype not in _DTYPE:
-        raise TypeError("%s must be float32, bfloat16 or float16 (got %s)" % (name, t.dtype))
-    return _DTYPE[t.dtype]
+def _wrong_type(name, t):
+    raise TypeError("%s must be float32, bfloat16 or float16 (got %s)" % (name, t))
 
 
-def _place(device, **more):
-    """The GPU index of `device`, after checking that every other tensor lives there too."""
-    if device.type != "cuda":
-        raise ValueError("the operators run on a GPU (got a tensor on %s)" % device)
-    for name, t in more.items():
-        if t is not None and t.device != device:
-            raise ValueError("%s is on %s, not on %s" % (name, t.device, device))
-    return device.index
+def _wrong_place(dev, **tensors):
+    """Names the tensor that is not on GPU number `dev` (-1: not on a GPU)."""
+    if dev < 0:
+        raise ValueError("the operators run on a GPU (got tensors on the host)")
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != dev:
+            raise ValueError("%s is on %s, not on cuda:%d" % (name, t.device, dev))
 
 
 class MX4(object):
@@ -46,12 +47,13 @@ class MX4(object):
     __slots__ = ("codes", "scales", "cols")
 
     def __init__(self, codes, scales, cols):
-        kp = -(-cols // 128) * 128
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        kb = (cols + 127) // 128 * 4
+        shape = codes.shape
+        if codes.dtype != _U8 or scales.dtype != _U8:
             raise TypeError("codes and scales must be uint8")
-        if codes.dim() != 2 or codes.shape[1] * 2 != kp or tuple(scales.shape) != (codes.shape[0], kp // 32):
+        if len(shape) != 2 or cols < 1 or shape[1] != 16 * kb or scales.shape != (shape[0], kb):
             raise ValueError("codes %s and scales %s do not hold %d columns: (rows, %d) and (rows, %d) are wanted"
-                             % (tuple(codes.shape), tuple(scales.shape), cols, kp // 2, kp // 32))
+                             % (tuple(shape), tuple(scales.shape), cols, 16 * kb, kb))
         if not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("codes and scales must be contiguous")
         self.codes, self.scales, self.cols = codes, scales, cols
@@ -68,64 +70,82 @@ class MX4(object):
         return "MX4(%d x %d on %s)" % (self.rows, self.cols, self.device)
 
 
+def _made(codes, scales, cols):         # an MX4 of tensors made here
+    q = MX4.__new__(MX4)
+    q.codes, q.scales, q.cols = codes, scales, cols
+    return q
+
+
 def mx4_quantize(x, axis=-1):
     """`x` (two dimensions, any strides) in 4 bits, blocks along `axis`: axis 1 keeps its rows, axis 0 gives a row per column of x (the
     form in which a weight stored (inputs, outputs) is multiplied)."""
+    dtype = _DTYPE.get(x.dtype)
+    if dtype is None:
+        _wrong_type("x", x.dtype)
     if x.dim() != 2:
         raise ValueError("x must have two dimensions")
-    dtype, dev = _float(x, "x"), _place(x.device)
     if axis not in (-2, -1, 0, 1):
         raise ValueError("axis must be 0 or 1")
+    dev = x.get_device()
+    if dev < 0:
+        _wrong_place(dev)
     (rows, cols), (rs, cs) = x.shape, x.stride()
     if axis in (0, -2):
         rows, cols, rs, cs = cols, rows, cs, rs
-    kp = -(-cols // 128) * 128
-    codes = torch.empty((rows, kp // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, kp // 32), dtype=torch.uint8, device=x.device)
+    kb = (cols + 127) // 128 * 4
+    device = x.device
+    codes = _empty((rows, 16 * kb), dtype=_U8, device=device)
+    scales = _empty((rows, kb), dtype=_U8, device=device)
     rc = _native.load_library().stattn_mx4_quantize(dev, _raw_stream(dev), x.data_ptr(), dtype, rows, cols, rs, cs, codes.data_ptr(), scales.data_ptr())
     if rc:
         _fail(rc)
-    return MX4(codes, scales, cols)
+    return _made(codes, scales, cols)
 
 
 def mx4_dequantize(q, dtype=torch.float32):
     """The numbers `q` stands for, (rows, cols) of `dtype`."""
-    if dtype not in _DTYPE:
-        raise TypeError("dtype must be float32, bfloat16 or float16 (got %s)" % dtype)
-    dev = _place(q.codes.device, scales=q.scales)
-    out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.codes.device)
-    rc = _native.load_library().stattn_mx4_dequantize(dev, _raw_stream(dev), q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols,
-                                                      out.data_ptr(), _DTYPE[dtype], q.cols)
+    t = _DTYPE.get(dtype)
+    if t is None:
+        _wrong_type("dtype", dtype)
+    codes, scales, cols = q.codes, q.scales, q.cols
+    dev = codes.get_device()
+    if dev < 0 or scales.get_device() != dev:
+        _wrong_place(dev, scales=scales)
+    rows = codes.shape[0]
+    out = _empty((rows, cols), dtype=dtype, device=codes.device)
+    rc = _native.load_library().stattn_mx4_dequantize(dev, _raw_stream(dev), codes.data_ptr(), scales.data_ptr(), rows, cols, out.data_ptr(), t, cols)
     if rc:
         _fail(rc)
     return out
 
 
-def _bias(bias, n, device):
-    if bias is None:
-        return None
-    if bias.dtype != torch.float32:
+def _check_bias(bias, n, dev):
+    if bias.dtype != _F32:
         raise TypeError("bias must be float32 (got %s)" % bias.dtype)
-    if bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous():
+    if bias.shape != (n,) or not bias.is_contiguous():
         raise ValueError("bias must be a contiguous vector of %d values" % n)
-    if bias.device != device:
-        raise ValueError("bias is on %s, not on %s" % (bias.device, device))
+    if bias.get_device() != dev:
+        _wrong_place(dev, bias=bias)
     return bias.data_ptr()
 
 
 def mx4_matmul(a, w, bias=None, dtype=torch.float32):
     """a (m, k) times w (n, k) transposed, both MX4, plus bias (n,) float32: (m, n) of `dtype`."""
-    if dtype not in _DTYPE:
-        raise TypeError("dtype must be float32, bfloat16 or float16 (got %s)" % dtype)
-    if a.cols != w.cols:
-        raise ValueError("inner dimensions differ: %d and %d" % (a.cols, w.cols))
-    device = a.codes.device
-    dev = _place(device, a_scales=a.scales, w=w.codes, w_scales=w.scales)
-    m, n = a.codes.shape[0], w.codes.shape[0]
-    b = _bias(bias, n, device)
-    y = torch.empty((m, n), dtype=dtype, device=device)
-    rc = _native.load_library().stattn_mx4_matmul(dev, _raw_stream(dev), a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(),
-                                                  w.scales.data_ptr(), m, n, a.cols, b, y.data_ptr(), _DTYPE[dtype], n)
+    t = _DTYPE.get(dtype)
+    if t is None:
+        _wrong_type("dtype", dtype)
+    k = a.cols
+    if k != w.cols:
+        raise ValueError("inner dimensions differ: %d and %d" % (k, w.cols))
+    ac, as_, wc, ws = a.codes, a.scales, w.codes, w.scales
+    dev = ac.get_device()
+    if dev < 0 or as_.get_device() != dev or wc.get_device() != dev or ws.get_device() != dev:
+        _wrong_place(dev, a_scales=as_, w=wc, w_scales=ws)
+    m, n = ac.shape[0], wc.shape[0]
+    b = None if bias is None else _check_bias(bias, n, dev)
+    y = _empty((m, n), dtype=dtype, device=ac.device)
+    rc = _native.load_library().stattn_mx4_matmul(dev, _raw_stream(dev), ac.data_ptr(), as_.data_ptr(), wc.data_ptr(), ws.data_ptr(), m, n, k, b,
+                                                  y.data_ptr(), t, n)
     if rc:
         _fail(rc)
     return y
@@ -134,23 +154,31 @@ def mx4_matmul(a, w, bias=None, dtype=torch.float32):
 def mx4_linear(x, w, bias=None):
     """x (m, k) -- its rows may be strided, its columns not -- rounded to 4 bits on the way, times w (n, k) MX4 transposed, plus bias
     (n,) float32: (m, n) of x's type."""
-    dtype = _float(x, "x")
-    if x.dim() != 2 or x.shape[1] != w.cols:
-        raise ValueError("x must be (m, %d), got %s" % (w.cols, tuple(x.shape)))
-    m, k = x.shape
-    ld = x.stride(0) if m > 1 else k
-    if (k > 1 and x.stride(1) != 1) or ld < k:
+    dtype = _DTYPE.get(x.dtype)
+    if dtype is None:
+        _wrong_type("x", x.dtype)
+    shape, k = x.shape, w.cols
+    if len(shape) != 2 or shape[1] != k:
+        raise ValueError("x must be (m, %d), got %s" % (k, tuple(shape)))
+    m = shape[0]
+    ld, one = x.stride()
+    if m <= 1:
+        ld = k
+    if (k > 1 and one != 1) or ld < k:
         raise ValueError("the columns of x must be contiguous and its rows must not overlap")
-    device = x.device
-    dev = _place(device, w=w.codes, w_scales=w.scales)
-    n = w.codes.shape[0]
-    b = _bias(bias, n, device)
+    wc, ws = w.codes, w.scales
+    dev = x.get_device()
+    if dev < 0 or wc.get_device() != dev or ws.get_device() != dev:
+        _wrong_place(dev, w=wc, w_scales=ws)
+    n = wc.shape[0]
+    b = None if bias is None else _check_bias(bias, n, dev)
     lib = _native.load_library()
-    y = torch.empty((m, n), dtype=x.dtype, device=device)
+    device = x.device
+    y = _empty((m, n), dtype=x.dtype, device=device)
     need = lib.stattn_mx4_linear_workspace(m, n, k)
-    work = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-    rc = lib.stattn_mx4_linear(dev, _raw_stream(dev), x.data_ptr(), dtype, ld, w.codes.data_ptr(), w.scales.data_ptr(), m, n, k, b,
-                               y.data_ptr(), n, work.data_ptr() if need else None, need)
+    work = _empty((need,), dtype=_U8, device=device) if need else None        # alive until the launches are enqueued
+    rc = lib.stattn_mx4_linear(dev, _raw_stream(dev), x.data_ptr(), dtype, ld, wc.data_ptr(), ws.data_ptr(), m, n, k, b, y.data_ptr(), n,
+                               work.data_ptr() if need else None, need)
     if rc:
         _fail(rc)
     return y
@@ -161,37 +189,48 @@ def verify_draft(draft, target, proposal, accept_u, draw_u, lens=None):
     proposal (b, j, v) -- None for arg-max drafts -- probabilities of one floating type with contiguous words, accept_u (b, j) and
     draw_u (b,) float32 in [0, 1), lens (b,) int32 or None.  words (b, j + 1) int64: the kept words, the drawn one, then -1;
     accepted (b,) int32: how many were kept."""
-    dtype = _float(target, "target")
-    if target.dim() != 3 or target.shape[1] < 1:
+    dtype = _DTYPE.get(target.dtype)
+    if dtype is None:
+        _wrong_type("target", target.dtype)
+    shape = target.shape
+    if len(shape) != 3 or shape[1] < 1:
         raise ValueError("target must be (b, j + 1, v)")
-    b, j, v = target.shape
+    b, j, v = shape
     j -= 1
-    if draft.dtype != torch.int64 or accept_u.dtype != torch.float32 or draw_u.dtype != torch.float32:
+    if draft.dtype != _I64 or accept_u.dtype != _F32 or draw_u.dtype != _F32:
         raise TypeError("draft must be int64, accept_u and draw_u float32")
     if draft.shape != (b, j) or accept_u.shape != (b, j) or draw_u.shape != (b,):
         raise ValueError("draft and accept_u must be (%d, %d), draw_u (%d,)" % (b, j, b))
-    if v > 1 and target.stride(2) != 1 or j > 1 and (draft.stride(1) != 1 or accept_u.stride(1) != 1) or b > 1 and draw_u.stride(0) != 1:
+    tb, tj, tv = target.stride()
+    db, dj = draft.stride()
+    ub, uj = accept_u.stride()
+    if v > 1 and tv != 1 or j > 1 and (dj != 1 or uj != 1) or b > 1 and draw_u.stride(0) != 1:
         raise ValueError("the last dimension of target, draft, accept_u and draw_u must be contiguous")
-    pp = pb = pj = 0
+    pp, pb, pj = None, 0, 0
+    dev = target.get_device()
+    wrong = dev < 0 or draft.get_device() != dev or accept_u.get_device() != dev or draw_u.get_device() != dev
     if proposal is not None:
         if proposal.dtype != target.dtype:
             raise TypeError("proposal must have target's type (%s), got %s" % (target.dtype, proposal.dtype))
-        if proposal.shape != (b, j, v) or (v > 1 and proposal.stride(2) != 1):
+        pb, pj, pv = proposal.stride() if proposal.dim() == 3 else (0, 0, 0)
+        if proposal.shape != (b, j, v) or (v > 1 and pv != 1):
             raise ValueError("proposal must be (%d, %d, %d) with contiguous words" % (b, j, v))
-        pp, pb, pj = proposal.data_ptr(), proposal.stride(0), proposal.stride(1)
-    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (b,) or (b > 1 and lens.stride(0) != 1)):
-        raise ValueError("lens must be a contiguous int32 vector of %d values" % b)
+        pp = proposal.data_ptr()
+        wrong = wrong or proposal.get_device() != dev
+    pl = None
+    if lens is not None:
+        if lens.dtype != _I32 or lens.shape != (b,) or (b > 1 and lens.stride(0) != 1):
+            raise ValueError("lens must be a contiguous int32 vector of %d values" % b)
+        pl = lens.data_ptr()
+        wrong = wrong or lens.get_device() != dev
+    if wrong:
+        _wrong_place(dev, draft=draft, proposal=proposal, accept_u=accept_u, draw_u=draw_u, lens=lens)
     device = target.device
-    dev = _place(device, draft=draft, proposal=proposal, accept_u=accept_u, draw_u=draw_u, lens=lens)
-    lib = _native.load_library()
-    words = torch.empty((b, j + 1), dtype=torch.int64, device=device)
-    accepted = torch.empty((b,), dtype=torch.int32, device=device)
-    need = lib.stattn_verify_draft_workspace(b, j, v)
-    work = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-    rc = lib.stattn_verify_draft(dev, _raw_stream(dev), draft.data_ptr(), draft.stride(0), target.data_ptr(), target.stride(0),
-                                 target.stride(1), pp, pb, pj, dtype, accept_u.data_ptr(), accept_u.stride(0), draw_u.data_ptr(),
-                                 None if lens is None else lens.data_ptr(), b, j, v, words.data_ptr(), j + 1, accepted.data_ptr(),
-                                 work.data_ptr() if need else None, need)
+    words = _empty((b, j + 1), dtype=_I64, device=device)
+    accepted = _empty((b,), dtype=_I32, device=device)
+    rc = _native.load_library().stattn_verify_draft(dev, _raw_stream(dev), draft.data_ptr(), db, target.data_ptr(), tb, tj, pp, pb, pj, dtype,
+                                                    accept_u.data_ptr(), ub, draw_u.data_ptr(), pl, b, j, v, words.data_ptr(), j + 1,
+                                                    accepted.data_ptr())
     if rc:
         _fail(rc)
     return words, accepted
