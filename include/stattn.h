@@ -167,6 +167,18 @@ int stattn_sample_search(stattn_handle* h, int nvid, const float* ctxg, const fl
                          const float* ctxm, int T, int K, int maxlen,
                          int64_t* out_tokens, float* out_scores, int32_t* out_lens);
 
+/* The same draws -- a caption is a sample of the next-word distributions, the score the sum of its words' probabilities -- with the
+ * vocabulary projection out of the word loop: a copy of it in 4 bits (stattn_mx4_quantize of ff_logit_W, made on every call) drafts
+ * `draft` words (1 .. 8) one after the other on the decoder's own states, then ONE product with the full-precision matrix gives the
+ * distributions in front of all of them and behind the last, and stattn_verify_draft keeps as many drafts as make the caption a
+ * sample of those, plus one word drawn from them.  Between 1 and draft + 1 words a round, whatever the 4-bit copy is worth.
+ * 1 <= nvid <= 16; features as in stattn_sample_search; every precision.  `uniforms`: the numbers in [0, 1) that decide, host memory
+ * (maxlen, 2 * draft + 1, nvid) -- a round takes one row each for the draws of its drafts, for their checks and for the last word --
+ * or NULL: from the handle's seed and a per-call counter.  out_drafted / out_kept (nvid) or NULL: words drafted and kept, a caption. */
+int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl,
+                          const float* ctxm, int T, int K, int draft, int maxlen, const float* uniforms,
+                          int64_t* out_tokens, float* out_scores, int32_t* out_lens, int32_t* out_drafted, int32_t* out_kept);
+
 /* gen_sample's third and fourth return values (next_state, next_memory, :994) for the videos of the last
  * stattn_beam_search: out_h / out_c (nvid,k,D), the first out_rows[v] rows of video v are valid -- the state outputs of
  * the f_next call that ended the video's loop (every live hypothesis at that point), or the gathered states of the

@@ -61,6 +61,8 @@ _SIGNATURES = {
                                      _I64, _F, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "stattn_beam_final_state": (C.c_int, [_H, _F, _F, C.POINTER(C.c_int32)]),
     "stattn_sample_search": (C.c_int, [_H, C.c_int, _F, _F, _F, _F, C.c_int, C.c_int, C.c_int, _I64, _F, C.POINTER(C.c_int32)]),
+    "stattn_sample_drafted": (C.c_int, [_H, C.c_int, _F, _F, _F, _F, C.c_int, C.c_int, C.c_int, C.c_int, _F, _I64, _F, C.POINTER(C.c_int32),
+                                        C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "stattn_set_batch": (C.c_int, [_H, _I64, _F, C.c_int, C.c_int, _F, _F, _F, _F, _F, _F, C.c_int, C.c_int]),
     "stattn_host_alloc": (C.c_int, [C.c_size_t, C.POINTER(C.c_void_p)]),
     "stattn_host_free": (C.c_int, [C.c_void_p]),
@@ -527,6 +529,32 @@ class Decoder(object):
         self._chk(self._lib.stattn_sample_search(self._h, nvid, pg, pk, pl, pm, T, K, int(maxlen), tok.ctypes.data_as(_I64),
                                                  _fp(sc), ln.ctypes.data_as(C.POINTER(C.c_int32))))
         self._beam_shape = (nvid, 1)
+        return [(tok[v, :ln[v]].tolist(), float(sc[v])) for v in range(nvid)]
+
+    def sample_drafted(self, ctxg=None, ctxg_mask=None, ctxl=None, ctxm=None, draft=4, maxlen=30, resident=False, uniforms=None):
+        """sample_search with the vocabulary projection out of the word loop (stattn_sample_drafted): a 4-bit copy of it drafts `draft`
+        words at a time and the full-precision one checks them together.  The same return value, drawn from the same distributions; the
+        words drafted and kept of each caption are in `self.draft_counts`, two int32 vectors.  `uniforms` (maxlen, 2 * draft + 1, nvid)
+        float32 in [0, 1) makes the draws the caller's."""
+        if resident:
+            if getattr(self, "_staged", None) is None:
+                raise ValueError("sample_drafted(resident=True) needs beam_stage() first")
+            nvid, T, K = self._staged
+            pg = pk = pl = pm = None
+        else:
+            ctxg, ctxg_mask, ctxl, ctxm, nvid, T, K = self._beam_shapes(ctxg, ctxg_mask, ctxl, ctxm)
+            pg, pk, pl, pm = _fp(ctxg), _fp(ctxg_mask), _fp(ctxl), _fp(ctxm)
+        draft, maxlen = int(draft), int(maxlen)
+        if uniforms is not None:
+            uniforms = _f32(uniforms, "uniforms", (maxlen, 2 * draft + 1, nvid))
+        tok = np.empty((nvid, max(maxlen, 0)), np.int64); sc = np.empty((nvid,), np.float32); ln = np.empty((nvid,), np.int32)
+        counts = np.zeros((2, nvid), np.int32)
+        i32 = C.POINTER(C.c_int32)
+        self._chk(self._lib.stattn_sample_drafted(self._h, nvid, pg, pk, pl, pm, T, K, draft, maxlen, _fp(uniforms), tok.ctypes.data_as(_I64),
+                                                  _fp(sc), ln.ctypes.data_as(i32), counts[0].ctypes.data_as(i32), counts[1].ctypes.data_as(i32)))
+        if not resident:
+            self._staged = (nvid, T, K)
+        self.draft_counts = (counts[0], counts[1])
         return [(tok[v, :ln[v]].tolist(), float(sc[v])) for v in range(nvid)]
 
     def beam_final_state(self):

@@ -1,0 +1,191 @@
+// C ABI of libstattn.so: drafted sampling -- gen_sample(stochastic=True) (model_attention.py:863-918) with words drafted by a 4-bit copy of
+// the vocabulary projection (ff_logit, :703-705) and checked against the full-precision one, several at a time.
+//
+// The recurrent part of the decoder needs the words one after the other and is the same for draft and target: behind the same words both
+// see the same state, so the states of the drafted positions are kept and nothing of it runs twice.  What a round saves is the
+// projection: dim_word x n_words in fp32, read once for draft + 1 positions instead of once a word; the draft reads 17/32 byte an
+// element.  (20 000 words: 41 MB against 5.4.)
+#include "steps.h"
+#include "ops/ops.h"
+
+extern "C" {
+
+int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl, const float* ctxm, int T,
+                          int K, int draft, int maxlen, const float* uniforms, int64_t* out_tokens, float* out_scores, int32_t* out_lens,
+                          int32_t* out_drafted, int32_t* out_kept) {
+    const bool resident = !ctxg && !ctxg_mask && !ctxl && !ctxm;
+    if (!h || nvid < 1 || nvid > 16 || (!resident && (!ctxg || !ctxg_mask || !ctxl || !ctxm)) || T <= 0 || K <= 0 || draft < 1 || draft > 8 ||
+        maxlen < 1 || !out_tokens || !out_scores || !out_lens)
+        return fail(h, STATTN_EINVAL, "sample_drafted: bad argument (1 <= nvid <= 16, 1 <= draft <= 8, maxlen >= 1)");
+    HIPCHK(h, hipSetDevice(h->device));
+    if (!resident) CHK(stattn_beam_stage(h, nvid, ctxg, ctxg_mask, ctxl, ctxm, T, K));
+    else if (!h->bk_valid || h->bk_n != nvid || h->bk_T != T || h->bk_K != K)
+        return fail(h, STATTN_ESTATE, "sample_drafted: no staged videos of this shape (call stattn_beam_stage)");
+    const int D = h->D, E = h->E, V = h->V, Vp = h->Vp, M = nvid, P = draft + 1;      // P positions a round
+    const Weights& w = h->w;
+    hipStream_t s = h->stream;
+    HIPCHK(h, hipStreamSynchronize(s));      // (buffers may be reallocated below)
+
+    // --- the videos: projected once (f_init and the context projections)
+    CtxPtrs c{};
+    float *rawl, *rawm, *mG, *mean, *h0, *c0;
+    const size_t nG = (size_t)nvid * T * D, nLd = (size_t)nvid * T * K * D;
+    CHK(getbuf_t(h, "bs_G", nG, &c.G)); CHK(getbuf_t(h, "bs_rawl", (size_t)nvid * T * K * h->Fl, &rawl));
+    CHK(getbuf_t(h, "bs_rawm", (size_t)nvid * T * h->Fm, &rawm)); CHK(getbuf_t(h, "bs_mG", (size_t)nvid * T, &mG));
+    CHK(getbuf_t(h, "bs_L", nLd, &c.L)); CHK(getbuf_t(h, "bs_Mo", nG, &c.Mo)); CHK(getbuf_t(h, "bs_PG", nG, &c.PG));
+    CHK(getbuf_t(h, "bs_PL", nLd, &c.PL)); CHK(getbuf_t(h, "bs_PM", nG, &c.PM));
+    CHK(getbuf_t(h, "bs_LW", h->opt.lt_mode == 1 ? nLd : 1, &c.LW));
+    CHK(getbuf_t(h, "bs_mean", (size_t)nvid * D, &mean)); CHK(getbuf_t(h, "bs_h0", (size_t)nvid * D, &h0));
+    CHK(getbuf_t(h, "bs_c0", (size_t)nvid * D, &c0));
+    CHK(project_context(h, nvid, T, K, c.G, rawl, rawm, c));
+    CHK(init_state(h, nvid, T, c.G, mG, mean, h0, c0));
+
+    // --- buffers of a round
+    int* vid; int64_t *xs, *words; int32_t *acc, *acc1;
+    float *hs, *cs, *hd, *emb, *sproj, *preh, *dp, *al, *CL, *eg, *em, *elt, *plt, *ag, *am, *alt, *ctx, *a1, *lq, *q, *lg, *p, *ub;
+    uint8_t *hc, *hsc;
+    CHK(getbuf_t(h, "dr_vid", (size_t)M, &vid)); CHK(getbuf_t(h, "dr_xs", (size_t)P * M, &xs)); CHK(getbuf_t(h, "dr_words", (size_t)M * P, &words));
+    CHK(getbuf_t(h, "dr_acc", (size_t)M, &acc)); CHK(getbuf_t(h, "dr_acc1", (size_t)M, &acc1));
+    CHK(getbuf_t(h, "dr_hs", (size_t)P * M * D, &hs)); CHK(getbuf_t(h, "dr_cs", (size_t)P * M * D, &cs));
+    CHK(getbuf_t(h, "dr_hd", (size_t)M * D, &hd)); CHK(getbuf_t(h, "dr_emb", (size_t)M * E, &emb));
+    CHK(getbuf_t(h, "dr_sproj", (size_t)M * 4 * D, &sproj)); CHK(getbuf_t(h, "dr_preh", (size_t)M * 4 * D, &preh));
+    CHK(getbuf_t(h, "dr_dp", (size_t)M * 3 * D, &dp));
+    CHK(getbuf_t(h, "dr_al", (size_t)M * T * K, &al)); CHK(getbuf_t(h, "dr_CL", (size_t)M * T * D, &CL));
+    CHK(getbuf_t(h, "dr_eg", (size_t)M * T, &eg)); CHK(getbuf_t(h, "dr_em", (size_t)M * T, &em)); CHK(getbuf_t(h, "dr_elt", (size_t)M * T, &elt));
+    CHK(getbuf_t(h, "dr_plt", h->opt.lt_mode == 0 ? (size_t)M * T * D : 1, &plt));
+    CHK(getbuf_t(h, "dr_ag", (size_t)M * T, &ag)); CHK(getbuf_t(h, "dr_am", (size_t)M * T, &am)); CHK(getbuf_t(h, "dr_alt", (size_t)M * T, &alt));
+    CHK(getbuf_t(h, "dr_ctx", (size_t)M * D, &ctx)); CHK(getbuf_t(h, "dr_a1", (size_t)P * M * E, &a1));
+    CHK(getbuf_t(h, "dr_lq", (size_t)M * Vp, &lq)); CHK(getbuf_t(h, "dr_q", (size_t)draft * M * Vp, &q));
+    CHK(getbuf_t(h, "dr_lg", (size_t)P * M * Vp, &lg)); CHK(getbuf_t(h, "dr_p", (size_t)P * M * Vp, &p));
+    CHK(getbuf_t(h, "dr_head", (size_t)V * (mx4_kp(E) / 2), &hc)); CHK(getbuf_t(h, "dr_head_scales", (size_t)V * (mx4_kp(E) / 32), &hsc));
+    DraftState d{};
+    d.M = M; d.D = D; d.k = draft; d.maxlen = maxlen; d.x = xs;
+    CHK(getbuf_t(h, "dr_h", (size_t)M * D, &d.h)); CHK(getbuf_t(h, "dr_c", (size_t)M * D, &d.c)); CHK(getbuf_t(h, "dr_info", (size_t)M, &d.info));
+    CHK(getbuf_t(h, "dr_tokens", (size_t)M * maxlen, &d.tokens)); CHK(getbuf_t(h, "dr_u", (size_t)(2 * draft + 1) * M, &d.u));
+    const size_t nu = (size_t)maxlen * (2 * draft + 1) * M;
+    CHK(getbuf_t(h, "dr_uniforms", nu, &ub));
+    d.uniforms = ub;
+
+    // --- numbers of this call, the 4-bit head of the current parameters, the captions' beginnings
+    std::vector<float> drawn;
+    if (!uniforms) {
+        auto mix = [](uint64_t z) { z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull; z = (z ^ (z >> 27)) * 0x94D049BB133111EBull; return z ^ (z >> 31); };
+        const uint64_t seed = mix(h->seed * 0x9E3779B97F4A7C15ull + 0x632BE59BD9B4E019ull * (++h->draw));
+        drawn.resize(nu);
+        for (size_t i = 0; i < nu; ++i) drawn[i] = (float)(mix(seed + 0x9E3779B97F4A7C15ull * (i + 1)) >> 40) * (1.0f / 16777216.0f);
+        uniforms = drawn.data();
+    }
+    HIPCHK(h, hipMemcpy(ub, uniforms, nu * sizeof(float), hipMemcpyHostToDevice));
+    HIPCHK(h, launch_mx4_quantize(s, Mx4QuantArgs{w.Wo, OP_F32, V, E, 1, Vp, hc, hsc}));      // ff_logit_W is (dim_word, n_words)
+    HIPCHK(h, launch_iota(s, vid, M, 1));
+    HIPCHK(h, launch_fill(s, dp, 0.5f, (size_t)M * 3 * D));                                  // use_noise = 0 (:469-472)
+    HIPCHK(h, launch_draft_begin(s, d, h0, c0));
+
+    auto round = [&]() -> int {
+        for (int j = 0; j < P; ++j) {
+            // the state behind word j of the round, and the readout's first layer (:817-836) in front of the next word
+            HIPCHK(h, launch_embed(s, xs + (size_t)j * M, w.Wemb, emb, M, E, V, 0));
+            StepIO io{};
+            io.M = M; io.T = T; io.K = K; io.c = c; io.vid = vid;
+            io.h_prev = j ? hs + (size_t)(j - 1) * M * D : d.h; io.c_prev = j ? cs + (size_t)(j - 1) * M * D : d.c;
+            io.sproj = sproj; io.preh = preh; io.xproj = nullptr; io.emb = emb; io.dp = dp; io.mask = nullptr; io.d1 = nullptr;
+            io.alphal = al; io.CL = CL; io.eg = eg; io.em = em; io.elt = elt; io.plt = plt;
+            io.alphag = ag; io.alpham = am; io.alphalt = alt; io.csum = nullptr; io.sel = nullptr; io.ctx = ctx;
+            io.h_out = hs + (size_t)j * M * D; io.c_out = cs + (size_t)j * M * D; io.gates = nullptr; io.hd = hd; io.pn = nullptr;
+            CHK(run_step(h, io));
+            SkArgs a{};
+            a.M = M; a.nseg = 1;
+            SkSeg& sg = a.seg[0];
+            skinny_seg_defaults(sg);
+            sg.npairs = 1; sg.p[0] = SkPair{hd, w.Wl1, D, E, D, 0};
+            if (h->opt.ctx2out) { sg.p[1] = SkPair{ctx, w.Wl2, D, E, D, 0}; sg.npairs = 2; sg.bias2 = w.bl2; }
+            sg.bias = w.bl1;
+            if (h->opt.prev2out) { sg.add = emb; sg.ldadd = E; }
+            float* aj = a1 + (size_t)j * M * E;
+            sg.act = 1; sg.scale = 0.5f; sg.C = aj; sg.ldc = E; sg.N = E;
+            HIPCHK(h, launch_skinny(s, a));
+            if (j == draft) break;
+            // the draft's distribution (4-bit head) and a word drawn from it: a check of no words draws from its target
+            float* qj = q + (size_t)j * M * Vp;
+            HIPCHK(h, launch_mx4_linear_few(s, Mx4LinearArgs{aj, OP_F32, M, E, Mx4View{hc, hsc, V, E}, w.bo, lq, Vp}));
+            HIPCHK(h, launch_softmax_nll(s, lq, Vp, qj, Vp, nullptr, nullptr, nullptr, M, V));
+            VerifyArgs draw{};
+            draw.target = qj; draw.target_b = Vp; draw.type = OP_F32; draw.draw_u = d.u + (size_t)j * M; draw.b = M; draw.j = 0; draw.v = V;
+            draw.words = xs + (size_t)(j + 1) * M; draw.words_ld = 1; draw.accepted = acc1;
+            HIPCHK(h, launch_verify_draft(s, draw));
+        }
+        // the full-precision distributions of all positions at once (:703-709), the check, the captions
+        if (P * M <= 64) {
+            SkArgs b{};
+            b.M = P * M; b.nseg = 1;
+            SkSeg& so = b.seg[0];
+            skinny_seg_defaults(so);
+            so.npairs = 1; so.p[0] = SkPair{a1, w.Wo, E, Vp, E, 0};
+            so.bias = w.bo; so.C = lg; so.ldc = Vp; so.N = Vp;
+            HIPCHK(h, launch_skinny(s, b));
+        } else {
+            GemmArgs g;
+            gemm_defaults(g); g.split = h->opt.precision != 0;
+            g.A = a1; g.lda = E; g.B = w.Wo; g.ldb = Vp; g.C = lg; g.ldc = Vp; g.M = P * M; g.N = Vp; g.K = E; g.bias = w.bo;
+            HIPCHK(h, launch_gemm(s, g, false, false));
+        }
+        HIPCHK(h, launch_softmax_nll(s, lg, Vp, p, Vp, nullptr, nullptr, nullptr, P * M, V));
+        VerifyArgs v{};
+        v.draft = xs + M; v.draft_b = 1; v.draft_j = M;
+        v.target = p; v.target_b = Vp; v.target_j = (int64_t)M * Vp; v.proposal = q; v.proposal_b = Vp; v.proposal_j = (int64_t)M * Vp;
+        v.type = OP_F32; v.accept_u = d.u + (size_t)draft * M; v.accept_b = 1; v.accept_j = M; v.draw_u = d.u + (size_t)2 * draft * M;
+        v.b = M; v.j = draft; v.v = V; v.words = words; v.words_ld = P; v.accepted = acc;
+        HIPCHK(h, launch_verify_draft(s, v));
+        HIPCHK(h, launch_draft_commit(s, d, words, acc, hs, cs, p, Vp));
+        return STATTN_OK;
+    };
+
+    // A round is some ten launches a word, each a few microseconds: captured once and replayed while the buffers and shapes stay the same.
+    // Falls back to plain launches if the capture is refused (and under profiling, whose events a graph would not time).
+    hipGraphExec_t ge = nullptr;
+    std::vector<uintptr_t> sig = {(uintptr_t)nvid, (uintptr_t)T, (uintptr_t)K, (uintptr_t)draft, (uintptr_t)maxlen, (uintptr_t)s};
+    for (const void* b : {(const void*)c.G, (const void*)c.L, (const void*)c.Mo, (const void*)c.PG, (const void*)c.PL, (const void*)c.PM, (const void*)c.LW,
+                          (const void*)vid, (const void*)xs, (const void*)words, (const void*)acc, (const void*)acc1, (const void*)hs, (const void*)cs,
+                          (const void*)hd, (const void*)emb, (const void*)sproj, (const void*)preh, (const void*)dp, (const void*)al, (const void*)CL,
+                          (const void*)eg, (const void*)em, (const void*)elt, (const void*)plt, (const void*)ag, (const void*)am, (const void*)alt,
+                          (const void*)ctx, (const void*)a1, (const void*)lq, (const void*)q, (const void*)lg, (const void*)p, (const void*)hc,
+                          (const void*)hsc, (const void*)d.h, (const void*)d.c, (const void*)d.info, (const void*)d.tokens, (const void*)d.u,
+                          (const void*)ub, (const void*)w.Wemb})
+        sig.push_back((uintptr_t)b);
+    if (!h->profiling && !sw_product("STATTN_BEAM_NOGRAPH")) {
+        if (h->draft_gexec && h->draft_gsig == sig) {
+            ge = h->draft_gexec;
+        } else {
+            if (h->draft_gexec) { (void)hipGraphExecDestroy(h->draft_gexec); h->draft_gexec = nullptr; }
+            hipGraph_t graph = nullptr;
+            bool ok = hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal) == hipSuccess;
+            if (ok) {
+                const int r = round();
+                const hipError_t e = hipStreamEndCapture(s, &graph);
+                ok = r == STATTN_OK && e == hipSuccess && graph && hipGraphInstantiate(&ge, graph, nullptr, nullptr, 0) == hipSuccess;
+            }
+            if (graph) (void)hipGraphDestroy(graph);
+            if (!ok) { ge = nullptr; (void)hipGetLastError(); }
+            h->draft_gexec = ge; h->draft_gsig = sig;
+        }
+    }
+    std::vector<DraftInfo> info(M);
+    for (int r = 0; r < maxlen; ++r) {       // every round adds a word at least to each caption that is not finished
+        if (ge) HIPCHK(h, hipGraphLaunch(ge, s));
+        else CHK(round());
+        HIPCHK(h, hipMemcpyAsync(info.data(), d.info, (size_t)M * sizeof(DraftInfo), hipMemcpyDeviceToHost, s));
+        HIPCHK(h, hipStreamSynchronize(s));
+        bool live = false;
+        for (const DraftInfo& f : info) live = live || !f.done;
+        if (!live) break;
+    }
+    HIPCHK(h, hipMemcpy(out_tokens, d.tokens, (size_t)M * maxlen * sizeof(int64_t), hipMemcpyDeviceToHost));
+    for (int m = 0; m < M; ++m) {
+        out_scores[m] = info[m].score; out_lens[m] = info[m].len;
+        if (out_drafted) out_drafted[m] = info[m].drafted;
+        if (out_kept) out_kept[m] = info[m].kept;
+    }
+    return STATTN_OK;
+}
+
+}  // extern "C"

@@ -157,7 +157,7 @@ int stattn_verify_draft(int device, void* stream, const int64_t* draft, int64_t 
     if (!target || !draw_u || !words || !accepted || (j && (!draft || !accept_u))) return refuse(STATTN_EINVAL, "verify_draft: null argument");
     const OnDevice on(device);
     if (on.err != hipSuccess) return launched("verify_draft", on.err);
-    const VerifyArgs a{draft, draft_ld, target, target_b, target_j, proposal, proposal_b, proposal_j, (OpType)dtype, accept_u, accept_ld,
+    const VerifyArgs a{draft, draft_ld, 1, target, target_b, target_j, proposal, proposal_b, proposal_j, (OpType)dtype, accept_u, accept_ld, 1,
                        draw_u, lens, b, (int)j, v, words, words_ld, accepted};
     return launched("verify_draft", launch_verify_draft(static_cast<hipStream_t>(stream), a));
 }

@@ -138,6 +138,9 @@ struct stattn_handle {
     hipGraphExec_t beam_gexec_last = nullptr;   // two words, the second one the LAST of a search (no attention launch for a word that never comes)
     hipGraphExec_t beam_gexec8 = nullptr;   // eight words: a replay costs 10-16 us of launch overhead whatever it holds
     std::vector<uintptr_t> beam_gsig;
+    // drafted sampling: one round (all launches between two looks at the captions), kept the same way
+    hipGraphExec_t draft_gexec = nullptr;
+    std::vector<uintptr_t> draft_gsig;
     long beam_graph_replays = 0;        // replays in the last stattn_beam_search (0 = eager launches)
     // which code path the decoder steps took (stattn_dbg_counter 1..4; reset by stattn_forward_train / stattn_backward):
     // forward steps whose attention launch carried the h.U rider, forward steps on the row-panel kernels, reverse steps

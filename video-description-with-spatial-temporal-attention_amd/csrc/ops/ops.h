@@ -44,16 +44,30 @@ struct Mx4LinearArgs {
 hipError_t launch_mx4_linear_few(hipStream_t s, const Mx4LinearArgs& a);
 
 struct VerifyArgs {
-    const int64_t* draft; int64_t draft_ld;
+    const int64_t* draft; int64_t draft_b, draft_j;          // strides as below
     const void* target; int64_t target_b, target_j;          // strides of the caption and of the position, in elements
     const void* proposal; int64_t proposal_b, proposal_j;    // or null: every drafted word was certain
     OpType type;
-    const float* accept_u; int64_t accept_ld;
+    const float* accept_u; int64_t accept_b, accept_j;
     const float* draw_u;
     const int32_t* lens;                                     // or null: every draft has j words
     int64_t b; int j; int64_t v;
     int64_t* words; int64_t words_ld; int32_t* accepted;
 };
 hipError_t launch_verify_draft(hipStream_t s, const VerifyArgs& a);
+
+// drafted sampling (api_draft.cpp): what is kept of each caption between rounds of k drafted words
+struct DraftInfo { int len, done, rounds, drafted, kept; float score; };
+struct DraftState {
+    int M, D, k, maxlen;
+    float* h; float* c; int64_t* x;      // state and last word in front of the next round
+    DraftInfo* info;
+    int64_t* tokens;                     // [M][maxlen]
+    const float* uniforms;               // [maxlen][2 k + 1][M]: draws of the drafts, checks, draw of the last word
+    float* u;                            // [2 k + 1][M] of the round to come
+};
+hipError_t launch_draft_begin(hipStream_t s, const DraftState& d, const float* h0, const float* c0);
+hipError_t launch_draft_commit(hipStream_t s, const DraftState& d, const int64_t* words, const int32_t* accepted, const float* hs, const float* cs,
+                               const float* p, int64_t ldp);
 
 }  // namespace stattn

@@ -93,7 +93,8 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
     __shared__ double part[2][2][NW];       // [turn][level]: never written again while a wave may still read it
     const int64_t i = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t* draft = a.draft + i * a.draft_ld;
+    const int64_t* drafts = a.draft + i * a.draft_b;
+    auto draft = [&](int j) { return drafts[j * a.draft_j]; };
     // every wave finds the first refused word for itself, a lane a word
     const int len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j;
     int n = len;
@@ -101,12 +102,12 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
         const int j = j0 + lane;
         bool kept = true;
         if (j < len) {
-            const int64_t d = draft[j];
+            const int64_t d = draft(j);
             kept = d >= 0 && d < a.v;
             if (kept) {
                 const double p = prob<T>(a.target, i * a.target_b + j * a.target_j + d);
                 const double q = a.proposal ? prob<T>(a.proposal, i * a.proposal_b + j * a.proposal_j + d) : 1.0;
-                kept = (double)a.accept_u[i * a.accept_ld + j] * q < p;
+                kept = (double)a.accept_u[i * a.accept_b + j * a.accept_j] * q < p;
             }
         }
         const unsigned long long refused = __ballot(!kept);
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
     w.v = a.v;
     w.p = static_cast<const E*>(a.target) + i * a.target_b + n * a.target_j;
     w.q = n < len && a.proposal ? static_cast<const E*>(a.proposal) + i * a.proposal_b + n * a.proposal_j : nullptr;
-    w.certain = n < len && !a.proposal ? draft[n] : -1;
+    w.certain = n < len && !a.proposal ? draft(n) : -1;
     const double u = (double)a.draw_u[i];
 
     int64_t word = -1;
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
         w.q = nullptr; w.certain = -1;       // nothing is left over a proposal that is nowhere smaller: the draw is from p itself
     }
     if (wave == 0)
-        for (int k = lane; k <= a.j; k += 64) a.words[i * a.words_ld + k] = k < n ? draft[k] : k == n ? word : -1;
+        for (int k = lane; k <= a.j; k += 64) a.words[i * a.words_ld + k] = k < n ? draft(k) : k == n ? word : -1;
     if (tid == 0) a.accepted[i] = n;
 }
 

@@ -593,6 +593,18 @@ class Attention(object):
         dec = self._bind(tparams, options)
         return dec.beam_search(ctxgs, ctxg_masks, ctxls, ctxms, k=k, maxlen=maxlen, suppress_eos=suppress_eos)
 
+    def gen_sample_drafted(self, tparams, options, ctxgs, ctxg_masks, ctxls, ctxms, draft=4, maxlen=30, uniforms=None):
+        """gen_sample(stochastic=True) (model_attention.py:863-918) for a batch of videos, with words drafted by a 4-bit copy of the
+        vocabulary projection and checked by the full-precision one, several at a time (Decoder.sample_drafted): [(sample, score), ...]
+        per video, samples of the same distributions.  Any number of videos; sixteen go through the device together."""
+        dec = self._bind(tparams, options)
+        out = []
+        for v in range(0, len(ctxgs), 16):
+            part = slice(v, v + 16)
+            u = None if uniforms is None else numpy.ascontiguousarray(uniforms[:, :, part])
+            out += dec.sample_drafted(ctxgs[part], ctxg_masks[part], ctxls[part], ctxms[part], draft=draft, maxlen=maxlen, uniforms=u)
+        return out
+
     # ---------------------------------------------------------------- teacher-forced scoring
     def pred_probs(self, batches, f_log_probs, verbose=False):
         """Teacher-forced scoring of a split with the contract of model_attention.py:996-1032: f_log_probs returns -cost
