@@ -41,11 +41,11 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
     CHK(init_state(h, nvid, T, c.G, mG, mean, h0, c0));
 
     // --- buffers of a round
-    int* vid; int64_t *xs, *words; int32_t *acc, *acc1;
+    int* vid; int64_t *xs, *words; int32_t* acc;
     float *hs, *cs, *hd, *emb, *sproj, *preh, *dp, *al, *CL, *eg, *em, *elt, *plt, *ag, *am, *alt, *ctx, *a1, *lq, *q, *lg, *p, *ub;
     uint8_t *hc, *hsc;
     CHK(getbuf_t(h, "dr_vid", (size_t)M, &vid)); CHK(getbuf_t(h, "dr_xs", (size_t)P * M, &xs)); CHK(getbuf_t(h, "dr_words", (size_t)M * P, &words));
-    CHK(getbuf_t(h, "dr_acc", (size_t)M, &acc)); CHK(getbuf_t(h, "dr_acc1", (size_t)M, &acc1));
+    CHK(getbuf_t(h, "dr_acc", (size_t)M, &acc));
     CHK(getbuf_t(h, "dr_hs", (size_t)P * M * D, &hs)); CHK(getbuf_t(h, "dr_cs", (size_t)P * M * D, &cs));
     CHK(getbuf_t(h, "dr_hd", (size_t)M * D, &hd)); CHK(getbuf_t(h, "dr_emb", (size_t)M * E, &emb));
     CHK(getbuf_t(h, "dr_sproj", (size_t)M * 4 * D, &sproj)); CHK(getbuf_t(h, "dr_preh", (size_t)M * 4 * D, &preh));
@@ -66,6 +66,16 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
     CHK(getbuf_t(h, "dr_uniforms", nu, &ub));
     d.uniforms = ub;
 
+    // On the row-panel kernels the readout launch of a word also leaves the state projections of its h, so the next word starts with its
+    // attention; the positions' projections are kept with their states.
+    FwdPanels pn{};
+    const bool panels = use_panels(h, M, 1) && Vp % 16 == 0;
+    float* projs = nullptr;
+    if (panels) {
+        CHK(pack_fwd_panels(h, &pn, true));
+        CHK(getbuf_t(h, "dr_projs", (size_t)P * M * 8 * D, &projs)); CHK(getbuf_t(h, "dr_proj", (size_t)M * 8 * D, &d.proj));
+    }
+
     // --- numbers of this call, the 4-bit head of the current parameters, the captions' beginnings
     std::vector<float> drawn;
     if (!uniforms) {
@@ -81,38 +91,64 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
     HIPCHK(h, launch_fill(s, dp, 0.5f, (size_t)M * 3 * D));                                  // use_noise = 0 (:469-472)
     HIPCHK(h, launch_draft_begin(s, d, h0, c0));
 
+    // state projections of h (M rows) into two segments behind `n` others of a row-panel launch
+    auto project = [&](PnArgs& a, int n, const float* hrows, float* to) {
+        a.M = M; a.nseg = n + 2;
+        for (int i = 0; i < 2; ++i) {
+            PnSeg& sp = a.seg[n + i];
+            pn_seg_defaults(sp);
+            sp.npairs = 1; sp.p[0] = PnPair{hrows, D, i == 0 ? pn.Wd : pn.U, D, 0};
+            sp.C = to + (size_t)i * 4 * D; sp.ldc = 8 * D; sp.N = 4 * D;
+        }
+    };
+    if (panels) {
+        PnArgs a{};
+        project(a, 0, d.h, d.proj);
+        HIPCHK(h, launch_panel(s, a));
+    }
     auto round = [&]() -> int {
         for (int j = 0; j < P; ++j) {
             // the state behind word j of the round, and the readout's first layer (:817-836) in front of the next word
-            HIPCHK(h, launch_embed(s, xs + (size_t)j * M, w.Wemb, emb, M, E, V, 0));
+            if (j == 0) HIPCHK(h, launch_embed(s, xs, w.Wemb, emb, M, E, V, 0));      // (later ones: by the draw)
             StepIO io{};
             io.M = M; io.T = T; io.K = K; io.c = c; io.vid = vid;
             io.h_prev = j ? hs + (size_t)(j - 1) * M * D : d.h; io.c_prev = j ? cs + (size_t)(j - 1) * M * D : d.c;
             io.sproj = sproj; io.preh = preh; io.xproj = nullptr; io.emb = emb; io.dp = dp; io.mask = nullptr; io.d1 = nullptr;
             io.alphal = al; io.CL = CL; io.eg = eg; io.em = em; io.elt = elt; io.plt = plt;
             io.alphag = ag; io.alpham = am; io.alphalt = alt; io.csum = nullptr; io.sel = nullptr; io.ctx = ctx;
-            io.h_out = hs + (size_t)j * M * D; io.c_out = cs + (size_t)j * M * D; io.gates = nullptr; io.hd = hd; io.pn = nullptr;
+            io.h_out = hs + (size_t)j * M * D; io.c_out = cs + (size_t)j * M * D; io.gates = nullptr; io.hd = hd;
+            if (panels) {
+                io.pn = &pn; io.skip_hproj = true; io.ldproj = 8 * D;
+                io.sproj = j ? projs + (size_t)(j - 1) * M * 8 * D : d.proj;
+                io.preh = io.sproj + (size_t)4 * D;
+            }
             CHK(run_step(h, io));
-            SkArgs a{};
-            a.M = M; a.nseg = 1;
-            SkSeg& sg = a.seg[0];
-            skinny_seg_defaults(sg);
-            sg.npairs = 1; sg.p[0] = SkPair{hd, w.Wl1, D, E, D, 0};
-            if (h->opt.ctx2out) { sg.p[1] = SkPair{ctx, w.Wl2, D, E, D, 0}; sg.npairs = 2; sg.bias2 = w.bl2; }
-            sg.bias = w.bl1;
-            if (h->opt.prev2out) { sg.add = emb; sg.ldadd = E; }
             float* aj = a1 + (size_t)j * M * E;
-            sg.act = 1; sg.scale = 0.5f; sg.C = aj; sg.ldc = E; sg.N = E;
-            HIPCHK(h, launch_skinny(s, a));
+            auto readout = [&](auto& sg) {
+                if (h->opt.ctx2out) { sg.npairs = 2; sg.bias2 = w.bl2; }
+                sg.bias = w.bl1;
+                if (h->opt.prev2out) { sg.add = emb; sg.ldadd = E; }
+                sg.act = 1; sg.scale = 0.5f; sg.C = aj; sg.ldc = E; sg.N = E;
+            };
+            if (panels) {
+                PnArgs a{};
+                pn_seg_defaults(a.seg[0]);
+                a.seg[0].npairs = 1; a.seg[0].p[0] = PnPair{hd, D, pn.Wl1, D, 0}; a.seg[0].p[1] = PnPair{ctx, D, pn.Wl2, D, 0};
+                readout(a.seg[0]);
+                project(a, 1, hs + (size_t)j * M * D, projs + (size_t)j * M * 8 * D);
+                HIPCHK(h, launch_panel(s, a));
+            } else {
+                SkArgs a{};
+                a.M = M; a.nseg = 1;
+                skinny_seg_defaults(a.seg[0]);
+                a.seg[0].npairs = 1; a.seg[0].p[0] = SkPair{hd, w.Wl1, D, E, D, 0}; a.seg[0].p[1] = SkPair{ctx, w.Wl2, D, E, D, 0};
+                readout(a.seg[0]);
+                HIPCHK(h, launch_skinny(s, a));
+            }
             if (j == draft) break;
-            // the draft's distribution (4-bit head) and a word drawn from it: a check of no words draws from its target
-            float* qj = q + (size_t)j * M * Vp;
+            // the draft's distribution (4-bit head), a word drawn from it, that word's embedding
             HIPCHK(h, launch_mx4_linear_few(s, Mx4LinearArgs{aj, OP_F32, M, E, Mx4View{hc, hsc, V, E}, w.bo, lq, Vp}));
-            HIPCHK(h, launch_softmax_nll(s, lq, Vp, qj, Vp, nullptr, nullptr, nullptr, M, V));
-            VerifyArgs draw{};
-            draw.target = qj; draw.target_b = Vp; draw.type = OP_F32; draw.draw_u = d.u + (size_t)j * M; draw.b = M; draw.j = 0; draw.v = V;
-            draw.words = xs + (size_t)(j + 1) * M; draw.words_ld = 1; draw.accepted = acc1;
-            HIPCHK(h, launch_verify_draft(s, draw));
+            HIPCHK(h, launch_softmax_draw(s, DrawArgs{lq, q + (size_t)j * M * Vp, Vp, V, M, d.u + (size_t)j * M, xs + (size_t)(j + 1) * M, w.Wemb, emb, E}));
         }
         // the full-precision distributions of all positions at once (:703-709), the check, the captions
         if (P * M <= 64) {
@@ -129,28 +165,29 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
             g.A = a1; g.lda = E; g.B = w.Wo; g.ldb = Vp; g.C = lg; g.ldc = Vp; g.M = P * M; g.N = Vp; g.K = E; g.bias = w.bo;
             HIPCHK(h, launch_gemm(s, g, false, false));
         }
-        HIPCHK(h, launch_softmax_nll(s, lg, Vp, p, Vp, nullptr, nullptr, nullptr, P * M, V));
+        HIPCHK(h, launch_softmax_draw(s, DrawArgs{lg, p, Vp, V, P * M, nullptr, nullptr, nullptr, nullptr, 0}));
         VerifyArgs v{};
         v.draft = xs + M; v.draft_b = 1; v.draft_j = M;
         v.target = p; v.target_b = Vp; v.target_j = (int64_t)M * Vp; v.proposal = q; v.proposal_b = Vp; v.proposal_j = (int64_t)M * Vp;
         v.type = OP_F32; v.accept_u = d.u + (size_t)draft * M; v.accept_b = 1; v.accept_j = M; v.draw_u = d.u + (size_t)2 * draft * M;
         v.b = M; v.j = draft; v.v = V; v.words = words; v.words_ld = P; v.accepted = acc;
         HIPCHK(h, launch_verify_draft(s, v));
-        HIPCHK(h, launch_draft_commit(s, d, words, acc, hs, cs, p, Vp));
+        HIPCHK(h, launch_draft_commit(s, d, words, acc, hs, cs, panels ? projs : nullptr, p, Vp));
         return STATTN_OK;
     };
 
     // A round is some ten launches a word, each a few microseconds: captured once and replayed while the buffers and shapes stay the same.
     // Falls back to plain launches if the capture is refused (and under profiling, whose events a graph would not time).
     hipGraphExec_t ge = nullptr;
-    std::vector<uintptr_t> sig = {(uintptr_t)nvid, (uintptr_t)T, (uintptr_t)K, (uintptr_t)draft, (uintptr_t)maxlen, (uintptr_t)s};
+    std::vector<uintptr_t> sig = {(uintptr_t)nvid, (uintptr_t)T, (uintptr_t)K, (uintptr_t)draft, (uintptr_t)maxlen, (uintptr_t)panels, (uintptr_t)s};
     for (const void* b : {(const void*)c.G, (const void*)c.L, (const void*)c.Mo, (const void*)c.PG, (const void*)c.PL, (const void*)c.PM, (const void*)c.LW,
-                          (const void*)vid, (const void*)xs, (const void*)words, (const void*)acc, (const void*)acc1, (const void*)hs, (const void*)cs,
+                          (const void*)vid, (const void*)xs, (const void*)words, (const void*)acc, (const void*)hs, (const void*)cs,
                           (const void*)hd, (const void*)emb, (const void*)sproj, (const void*)preh, (const void*)dp, (const void*)al, (const void*)CL,
                           (const void*)eg, (const void*)em, (const void*)elt, (const void*)plt, (const void*)ag, (const void*)am, (const void*)alt,
                           (const void*)ctx, (const void*)a1, (const void*)lq, (const void*)q, (const void*)lg, (const void*)p, (const void*)hc,
                           (const void*)hsc, (const void*)d.h, (const void*)d.c, (const void*)d.info, (const void*)d.tokens, (const void*)d.u,
-                          (const void*)ub, (const void*)w.Wemb})
+                          (const void*)ub, (const void*)w.Wemb, (const void*)d.proj, (const void*)projs, (const void*)pn.Wd, (const void*)pn.U,
+                          (const void*)pn.Wc, (const void*)pn.W, (const void*)pn.Wl1, (const void*)pn.Wl2, (const void*)emb})
         sig.push_back((uintptr_t)b);
     if (!h->profiling && !sw_product("STATTN_BEAM_NOGRAPH")) {
         if (h->draft_gexec && h->draft_gsig == sig) {

@@ -1,7 +1,111 @@
-// Bookkeeping of drafted sampling (api_draft.cpp): per caption the state behind the kept words, the words, the next round's numbers.
-#include "ops.h"
+// Kernels of drafted sampling (api_draft.cpp): distributions and draws of the drafts, and per caption the state behind the kept words, the
+// words, the next round's numbers.
+#include "mx4_inl.h"
 
 namespace stattn {
+
+// One workgroup of 16 waves a row, a stretch of the row (a multiple of 512 words) for each wave, eight neighbours a lane.  Three walks of
+// it, the second and third from the caches: the largest logit, the sum, the probabilities -- whose own sums over the stretches (in 64 bits)
+// then say where a draw falls, and the first wave looks there word by word.  A row of 20000 words is 20 values a lane: what counts is the
+// chain of reads (the 256-lane softmax of the other paths takes 41 us for such a row, and the draw was another launch).
+__global__ __launch_bounds__(1024) void softmax_draw_kernel(DrawArgs a) {
+    constexpr int NW = 16;
+    __shared__ float top[NW], sums[NW];
+    __shared__ double part[NW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const float* x = a.logits + (int64_t)blockIdx.x * a.ld;
+    float* p = a.p + (int64_t)blockIdx.x * a.ld;
+    const int step = ((a.v + NW - 1) / NW + 511) & ~511, lo = min(wave * step, a.v), hi = min(lo + step, a.v);
+    auto walk = [&](auto each) {                       // each(first column, eight logits): -inf behind the row's end (in the row's padding)
+        for (int c = lo + 8 * lane; c < hi; c += 512) {
+            const float4 u = reinterpret_cast<const float4*>(x + c)[0], w = reinterpret_cast<const float4*>(x + c)[1];
+            float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j >= hi) v[j] = -INFINITY;
+            each(c, v);
+        }
+    };
+    float m = -INFINITY;
+    walk([&](int, const float* v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (lane == 0) top[wave] = m;
+    __syncthreads();
+    for (int k = 0; k < NW; ++k) m = fmaxf(m, top[k]);
+    float sum = 0.f;
+    walk([&](int, const float* v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += __expf(v[j] - m);
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int k = 0; k < NW; ++k) sum += sums[k];
+    const float inv = 1.0f / sum;
+    double mine = 0.0;
+    walk([&](int c, const float* v) {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { e[j] = __expf(v[j] - m) * inv; mine += (double)e[j]; }
+        reinterpret_cast<float4*>(p + c)[0] = make_float4(e[0], e[1], e[2], e[3]);     // (0 behind the row's end)
+        reinterpret_cast<float4*>(p + c)[1] = make_float4(e[4], e[5], e[6], e[7]);
+    });
+    if (!a.u) return;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
+    if (lane == 0) part[wave] = mine;
+    __syncthreads();
+    if (wave) return;
+    double total = 0.0;
+    for (int k = 0; k < NW; ++k) total += part[k];
+    const double t = (double)a.u[blockIdx.x] * total;
+    double c = 0.0, base = 0.0;
+    int hit = -1, last = 0;
+    for (int k = 0; k < NW; ++k) {
+        if (part[k] > 0.0 && hit < 0) {
+            last = k; base = c;
+            if (c + part[k] > t) hit = k;
+        }
+        c += part[k];
+    }
+    const int from = min(last * step, a.v), to = min(from + step, a.v);
+    int word = 0;                                       // (a row of NaNs draws word 0)
+    for (int c0 = from; c0 < to; c0 += 512) {
+        const int i = c0 + 8 * lane;
+        float e[8];
+        double own = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { e[j] = i + j < to ? p[i + j] : 0.f; own += (double)e[j]; }
+        double incl = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const double y = __shfl_up(incl, o, 64); if (lane >= o) incl += y; }
+        double run = base + (incl - own);
+        int first = -1, some = -1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            run += (double)e[j];
+            if (e[j] > 0.f) { some = i + j; if (run > t && first < 0) first = i + j; }
+        }
+        const unsigned long long over = __ballot(first >= 0), with = __ballot(some >= 0);
+        if (over) { word = __shfl(first, __builtin_ctzll(over), 64); break; }
+        if (with) word = __shfl(some, 63 - __builtin_clzll(with), 64);
+        base += __shfl(incl, 63, 64);
+    }
+    if (lane == 0) a.words[blockIdx.x] = word;
+    for (int i = lane; i < a.dim / 4; i += 64)
+        reinterpret_cast<float4*>(a.emb + (int64_t)blockIdx.x * a.dim)[i] = reinterpret_cast<const float4*>(a.Wemb + (int64_t)word * a.dim)[i];
+}
+
+hipError_t launch_softmax_draw(hipStream_t s, const DrawArgs& a) {
+    softmax_draw_kernel<<<dim3((unsigned)a.rows), 1024, 0, s>>>(a);
+    return hipGetLastError();
+}
 
 // A caption's share of the next round's uniform numbers: row r of a round holds one number a caption
 __device__ __forceinline__ void next_numbers(const DraftState& d, int m, int round) {
@@ -20,10 +124,10 @@ __global__ __launch_bounds__(256) void draft_begin_kernel(DraftState d, const fl
     next_numbers(d, m, 0);
 }
 
-// words row m: n = accepted[m] kept drafts, then the drawn word.  hs / cs hold the states behind each of the round's k + 1 inputs (the
-// last word, then the drafts), p the target's rows in front of each word.
+// words row m: n = accepted[m] kept drafts, then the drawn word.  hs / cs (and projs, 8 D wide) hold the states behind each of the round's
+// k + 1 inputs (the last word, then the drafts), p the target's rows in front of each word.
 __global__ __launch_bounds__(256) void draft_commit_kernel(DraftState d, const int64_t* words, const int32_t* accepted, const float* hs, const float* cs,
-                                                           const float* p, int64_t ldp) {
+                                                           const float* projs, const float* p, int64_t ldp) {
     const int m = blockIdx.x;
     DraftInfo f = d.info[m];
     __syncthreads();                       // (thread 0 writes it below)
@@ -32,6 +136,8 @@ __global__ __launch_bounds__(256) void draft_commit_kernel(DraftState d, const i
     const float* h = hs + ((int64_t)n * d.M + m) * d.D;
     const float* c = cs + ((int64_t)n * d.M + m) * d.D;
     for (int i = threadIdx.x; i < d.D; i += 256) { d.h[(int64_t)m * d.D + i] = h[i]; d.c[(int64_t)m * d.D + i] = c[i]; }
+    if (projs)
+        for (int i = threadIdx.x; i < 8 * d.D; i += 256) d.proj[(int64_t)m * 8 * d.D + i] = projs[((int64_t)n * d.M + m) * 8 * d.D + i];
     if (threadIdx.x == 0) {
         f.drafted += d.k; f.kept += n;
         int64_t w = 0;
@@ -54,8 +160,8 @@ hipError_t launch_draft_begin(hipStream_t s, const DraftState& d, const float* h
     return hipGetLastError();
 }
 hipError_t launch_draft_commit(hipStream_t s, const DraftState& d, const int64_t* words, const int32_t* accepted, const float* hs, const float* cs,
-                               const float* p, int64_t ldp) {
-    draft_commit_kernel<<<dim3((unsigned)d.M), 256, 0, s>>>(d, words, accepted, hs, cs, p, ldp);
+                               const float* projs, const float* p, int64_t ldp) {
+    draft_commit_kernel<<<dim3((unsigned)d.M), 256, 0, s>>>(d, words, accepted, hs, cs, projs, p, ldp);
     return hipGetLastError();
 }
 

@@ -61,6 +61,7 @@ struct DraftInfo { int len, done, rounds, drafted, kept; float score; };
 struct DraftState {
     int M, D, k, maxlen;
     float* h; float* c; int64_t* x;      // state and last word in front of the next round
+    float* proj;                         // [M][8 D] projections of h, or null
     DraftInfo* info;
     int64_t* tokens;                     // [M][maxlen]
     const float* uniforms;               // [maxlen][2 k + 1][M]: draws of the drafts, checks, draw of the last word
@@ -68,6 +69,13 @@ struct DraftState {
 };
 hipError_t launch_draft_begin(hipStream_t s, const DraftState& d, const float* h0, const float* c0);
 hipError_t launch_draft_commit(hipStream_t s, const DraftState& d, const int64_t* words, const int32_t* accepted, const float* hs, const float* cs,
-                               const float* p, int64_t ldp);
+                               const float* projs, const float* p, int64_t ldp);
+// Rows of probabilities p = softmax(logits); with `u` also a word drawn from each (the first whose running sum exceeds u * total) and its
+// embedding, `dim` floats.  ld: row stride of logits and p, a multiple of 8.
+struct DrawArgs {
+    const float* logits; float* p; int64_t ld; int v, rows;
+    const float* u; int64_t* words; const float* Wemb; float* emb; int dim;
+};
+hipError_t launch_softmax_draw(hipStream_t s, const DrawArgs& a);
 
 }  // namespace stattn
