@@ -323,12 +323,15 @@ int stattn_mx4_linear(int device, void* stream, const void* x_dev, int dtype, in
  * first whose running sum of weights exceeds draw_u * total, weights max(target - proposal, 0) at the refused position (target itself
  * if all of them are 0), or target behind a draft that was kept whole.  accepted[i] = kept words; words row i = the kept words, the
  * drawn one, -1 from there on.  The captions that result are samples of the target's distribution.  Products and sums are in 64 bits;
- * weights that are NaN count as 0; a drafted word outside [0, v) is refused; a row without any weight draws -1. */
+ * weights that are NaN count as 0; a drafted word outside [0, v) is refused; a row without any weight draws -1.
+ * `workspace_dev`: stattn_verify_draft_workspace(b, j, v) bytes, 16-byte aligned, overwritten (may be NULL when that is 0); not to be
+ * shared by calls that can run at the same time. */
+size_t stattn_verify_draft_workspace(int64_t b, int64_t j, int64_t v);
 int stattn_verify_draft(int device, void* stream, const int64_t* draft_dev, int64_t draft_ld, const void* target_dev,
                         int64_t target_stride_b, int64_t target_stride_j, const void* proposal_dev, int64_t proposal_stride_b,
                         int64_t proposal_stride_j, int dtype, const float* accept_u_dev, int64_t accept_ld, const float* draw_u_dev,
                         const int32_t* lens_dev, int64_t b, int64_t j, int64_t v, int64_t* words_dev, int64_t words_ld,
-                        int32_t* accepted_dev);
+                        int32_t* accepted_dev, void* workspace_dev, size_t workspace_bytes);
 
 /* ---- measurement hooks (bench.py's per-kernel rooflines) -------------------------------------------- */
 /* Average duration (ms) of the named kernel class over the last stattn_forward_train (or the stattn_beam_search /

@@ -72,8 +72,8 @@ def test_matmul_and_linear_refusals():
 def test_verify_refusals():
     f = lib().stattn_verify_draft
 
-    def call(b=2, j=3, v=10, dtype=0, draft=A, target=A, proposal=A, au=A, du=A, words=A, ld=4, acc=A):
-        return f(0, None, draft, j, target, (j + 1) * v, v, proposal, j * v, v, dtype, au, j, du, None, b, j, v, words, ld, acc)
+    def call(b=2, j=3, v=10, dtype=0, draft=A, target=A, proposal=A, au=A, du=A, words=A, ld=4, acc=A, ws=A, nws=1 << 30):
+        return f(0, None, draft, j, target, (j + 1) * v, v, proposal, j * v, v, dtype, au, j, du, None, b, j, v, words, ld, acc, ws, nws)
     refused(call(dtype=5), "dtype")
     refused(call(v=0), "v = 0")
     refused(call(j=-1), "j = -1")
@@ -82,6 +82,11 @@ def test_verify_refusals():
     refused(call(ld=3), "words_ld")
     for name in ("draft", "target", "au", "du", "words", "acc"):
         refused(call(**{name: None}), "null")
+    need = lib().stattn_verify_draft_workspace(2, 3, 200000)
+    assert need and not lib().stattn_verify_draft_workspace(2, 3, 20000)
+    refused(call(v=200000, nws=need - 1), "workspace")
+    refused(call(v=200000, ws=None), "workspace")
+    refused(call(v=200000, ws=A + 4), "workspace")
     assert call(b=0) == 0
 
 

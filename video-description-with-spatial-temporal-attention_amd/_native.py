@@ -91,7 +91,8 @@ _SIGNATURES = {
     "stattn_mx4_matmul": (C.c_int, [C.c_int, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, C.c_int, _I]),
     "stattn_mx4_linear_workspace": (C.c_size_t, [_I, _I, _I]),
     "stattn_mx4_linear": (C.c_int, [C.c_int, _P, _P, C.c_int, _I, _P, _P, _I, _I, _I, _P, _P, _I, _P, C.c_size_t]),
-    "stattn_verify_draft": (C.c_int, [C.c_int, _P, _P, _I, _P, _I, _I, _P, _I, _I, C.c_int, _P, _I, _P, _P, _I, _I, _I, _P, _I, _P]),
+    "stattn_verify_draft_workspace": (C.c_size_t, [_I, _I, _I]),
+    "stattn_verify_draft": (C.c_int, [C.c_int, _P, _P, _I, _P, _I, _I, _P, _I, _I, C.c_int, _P, _I, _P, _P, _I, _I, _I, _P, _I, _P, _P, C.c_size_t]),
     "stattn_set_profiling": (C.c_int, [_H, C.c_int]),
     "stattn_get_kernel_ms": (C.c_int, [_H, C.c_int, _F, C.POINTER(C.c_int)]),
 }

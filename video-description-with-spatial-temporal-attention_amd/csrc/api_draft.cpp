@@ -58,6 +58,8 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
     CHK(getbuf_t(h, "dr_lq", (size_t)M * Vp, &lq)); CHK(getbuf_t(h, "dr_q", (size_t)draft * M * Vp, &q));
     CHK(getbuf_t(h, "dr_lg", (size_t)P * M * Vp, &lg)); CHK(getbuf_t(h, "dr_p", (size_t)P * M * Vp, &p));
     CHK(getbuf_t(h, "dr_head", (size_t)V * (mx4_kp(E) / 2), &hc)); CHK(getbuf_t(h, "dr_head_scales", (size_t)V * (mx4_kp(E) / 32), &hsc));
+    double* vsums;
+    CHK(getbuf_t(h, "dr_sums", (size_t)M * verify_split(M, V) * 16, &vsums));
     DraftState d{};
     d.M = M; d.D = D; d.k = draft; d.maxlen = maxlen; d.x = xs;
     CHK(getbuf_t(h, "dr_h", (size_t)M * D, &d.h)); CHK(getbuf_t(h, "dr_c", (size_t)M * D, &d.c)); CHK(getbuf_t(h, "dr_info", (size_t)M, &d.info));
@@ -167,6 +169,7 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
         }
         HIPCHK(h, launch_softmax_draw(s, DrawArgs{lg, p, Vp, V, P * M, nullptr, nullptr, nullptr, nullptr, 0}));
         VerifyArgs v{};
+        v.split = verify_split(M, V); v.sums = vsums;
         v.draft = xs + M; v.draft_b = 1; v.draft_j = M;
         v.target = p; v.target_b = Vp; v.target_j = (int64_t)M * Vp; v.proposal = q; v.proposal_b = Vp; v.proposal_j = (int64_t)M * Vp;
         v.type = OP_F32; v.accept_u = d.u + (size_t)draft * M; v.accept_b = 1; v.accept_j = M; v.draw_u = d.u + (size_t)2 * draft * M;
@@ -186,7 +189,7 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
                           (const void*)eg, (const void*)em, (const void*)elt, (const void*)plt, (const void*)ag, (const void*)am, (const void*)alt,
                           (const void*)ctx, (const void*)a1, (const void*)lq, (const void*)q, (const void*)lg, (const void*)p, (const void*)hc,
                           (const void*)hsc, (const void*)d.h, (const void*)d.c, (const void*)d.info, (const void*)d.tokens, (const void*)d.u,
-                          (const void*)ub, (const void*)w.Wemb, (const void*)d.proj, (const void*)projs, (const void*)pn.Wd, (const void*)pn.U,
+                          (const void*)ub, (const void*)vsums, (const void*)w.Wemb, (const void*)d.proj, (const void*)projs, (const void*)pn.Wd, (const void*)pn.U,
                           (const void*)pn.Wc, (const void*)pn.W, (const void*)pn.Wl1, (const void*)pn.Wl2, (const void*)emb})
         sig.push_back((uintptr_t)b);
     if (!h->profiling && !sw_product("STATTN_BEAM_NOGRAPH")) {

@@ -143,10 +143,16 @@ int stattn_mx4_linear(int device, void* stream, const void* x, int dtype, int64_
     return launched("mx4_linear", launch_mx4_matmul(s, g));
 }
 
+size_t stattn_verify_draft_workspace(int64_t b, int64_t j, int64_t v) {
+    (void)j;
+    const int n = b > 0 ? verify_split(b, v) : 1;
+    return n > 1 ? (size_t)b * n * 16 * sizeof(double) : 0;
+}
+
 int stattn_verify_draft(int device, void* stream, const int64_t* draft, int64_t draft_ld, const void* target, int64_t target_b,
                         int64_t target_j, const void* proposal, int64_t proposal_b, int64_t proposal_j, int dtype, const float* accept_u,
                         int64_t accept_ld, const float* draw_u, const int32_t* lens, int64_t b, int64_t j, int64_t v, int64_t* words,
-                        int64_t words_ld, int32_t* accepted) {
+                        int64_t words_ld, int32_t* accepted, void* workspace, size_t workspace_bytes) {
     if (!type_ok(dtype)) return refuse(STATTN_EINVAL, "verify_draft: dtype %d is none of STATTN_F32, STATTN_BF16, STATTN_F16", dtype);
     if (b < 0 || b >= ((int64_t)1 << 22) || j < 0 || j > 65535 || v < 1 || v >= MAX_ROWS)
         return refuse(STATTN_EINVAL, "verify_draft: b = %lld, j = %lld, v = %lld are outside b < 2^22, 0 <= j < 2^16, 1 <= v < 2^31", (long long)b, (long long)j, (long long)v);
@@ -155,10 +161,13 @@ int stattn_verify_draft(int device, void* stream, const int64_t* draft, int64_t 
     if (words_ld < j + 1) return refuse(STATTN_EINVAL, "verify_draft: words_ld (%lld) must be at least j + 1", (long long)words_ld);
     if (!b) return STATTN_OK;
     if (!target || !draw_u || !words || !accepted || (j && (!draft || !accept_u))) return refuse(STATTN_EINVAL, "verify_draft: null argument");
+    const size_t need = stattn_verify_draft_workspace(b, j, v);
+    if (need && (!workspace || !al16(workspace) || workspace_bytes < need))
+        return refuse(STATTN_EINVAL, "verify_draft: a 16-byte aligned workspace of %zu bytes is needed (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
     const OnDevice on(device);
     if (on.err != hipSuccess) return launched("verify_draft", on.err);
     const VerifyArgs a{draft, draft_ld, 1, target, target_b, target_j, proposal, proposal_b, proposal_j, (OpType)dtype, accept_u, accept_ld, 1,
-                       draw_u, lens, b, (int)j, v, words, words_ld, accepted};
+                       draw_u, lens, b, (int)j, v, words, words_ld, accepted, verify_split(b, v), static_cast<double*>(workspace)};
     return launched("verify_draft", launch_verify_draft(static_cast<hipStream_t>(stream), a));
 }
 

@@ -62,30 +62,27 @@ __global__ __launch_bounds__(1024) void softmax_draw_kernel(DrawArgs a) {
     if (lane == 0) part[wave] = mine;
     __syncthreads();
     if (wave) return;
-    double total = 0.0;
-    for (int k = 0; k < NW; ++k) total += part[k];
-    const double t = (double)a.u[blockIdx.x] * total;
-    double c = 0.0, base = 0.0;
-    int hit = -1, last = 0;
-    for (int k = 0; k < NW; ++k) {
-        if (part[k] > 0.0 && hit < 0) {
-            last = k; base = c;
-            if (c + part[k] > t) hit = k;
-        }
-        c += part[k];
-    }
+    // the stretch that the draw falls into: a lane a stretch
+    const double own = lane < NW ? part[lane] : 0.0;
+    double upto = own;
+#pragma unroll
+    for (int o = 1; o < NW; o <<= 1) { const double y = __shfl_up(upto, o, 64); if (lane >= o) upto += y; }
+    const double t = (double)a.u[blockIdx.x] * __shfl(upto, NW - 1, 64);
+    const unsigned long long over16 = __ballot(lane < NW && own > 0.0 && upto > t), with16 = __ballot(own > 0.0);
+    const int last = over16 ? __builtin_ctzll(over16) : with16 ? 63 - __builtin_clzll(with16) : 0;
+    double base = __shfl(upto - own, last, 64);
     const int from = min(last * step, a.v), to = min(from + step, a.v);
     int word = 0;                                       // (a row of NaNs draws word 0)
     for (int c0 = from; c0 < to; c0 += 512) {
         const int i = c0 + 8 * lane;
         float e[8];
-        double own = 0.0;
+        double eight = 0.0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { e[j] = i + j < to ? p[i + j] : 0.f; own += (double)e[j]; }
-        double incl = own;
+        for (int j = 0; j < 8; ++j) { e[j] = i + j < to ? p[i + j] : 0.f; eight += (double)e[j]; }
+        double incl = eight;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) { const double y = __shfl_up(incl, o, 64); if (lane >= o) incl += y; }
-        double run = base + (incl - own);
+        double run = base + (incl - eight);
         int first = -1, some = -1;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {

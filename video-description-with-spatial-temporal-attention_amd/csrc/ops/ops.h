@@ -53,7 +53,17 @@ struct VerifyArgs {
     const int32_t* lens;                                     // or null: every draft has j words
     int64_t b; int j; int64_t v;
     int64_t* words; int64_t words_ld; int32_t* accepted;
+    int split; double* sums;                                 // workgroups that sum a caption's rows, and [b][split * 16] sums; 1: none
 };
+constexpr int VERIFY_SPLIT = 16;
+// Long rows of few captions: several workgroups a caption, up to two a CU in all.  (One takes 20 us for 128000 words; a launch more takes
+// the GPU 3 us and a caller 3.5, so rows under 32768 words stay with one.)
+inline int verify_split(int64_t b, int64_t v) {
+    if (v < 32768 || b > 256) return 1;
+    int n = 1;
+    while (n < VERIFY_SPLIT && b * n < 256 && v / (n * 32) >= 1024) n *= 2;
+    return n;
+}
 hipError_t launch_verify_draft(hipStream_t s, const VerifyArgs& a);
 
 // drafted sampling (api_draft.cpp): what is kept of each caption between rounds of k drafted words

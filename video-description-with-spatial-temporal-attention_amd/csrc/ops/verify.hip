@@ -18,23 +18,26 @@ __device__ __forceinline__ double wave_sum64(double v) {
     return v;
 }
 
-// One caption's weights over a stretch of the vocabulary.  q null: p alone, or p without the refused word (a certain proposal).
+// One caption's weights over a stretch of the vocabulary: p alone, p without the one word that a certain proposal has all its mass on, or
+// p over q.
 template <OpType T, bool WIDE>
 struct Weights {
     typedef typename Elem<T>::type E;
     const E* p;
-    const E* q;
-    int64_t v, certain;             // vocabulary; the word that a certain proposal has all its mass on, or -1
+    const E* q;                     // or null
+    int64_t certain;                // or -1
 
-    // p > q is decided in 32 bits, where it is exact (and false for a NaN); the difference is one operation in 64
-    __device__ __forceinline__ double of(float a, float b) const {
-        const bool over = a > b;
-        return (double)(over ? a : 0.f) - (double)(over ? b : 0.f);
+    // a > b is decided in 32 bits, where it is exact (and false for a NaN); the difference is one operation in 64
+    static __device__ __forceinline__ double over(float a, float b) {
+        const bool more = a > b;
+        return (double)(more ? a : 0.f) - (double)(more ? b : 0.f);
     }
-    __device__ __forceinline__ double at(int64_t i) const { return of((float)p[i], q ? (float)q[i] : i == certain ? 1.f : 0.f); }
+    static __device__ __forceinline__ double over(float a) { return (double)(a > 0.f ? a : 0.f); }
+    __device__ __forceinline__ double at(int64_t i) const { return q ? over((float)p[i], (float)q[i]) : i == certain ? over((float)p[i], 1.f) : over((float)p[i]); }
 
     // Sum of the weights from `from` to `to`, this lane's share of the wave's walk; K requests on their way.  The lanes take eight
-    // neighbours each where those are 16-byte loads, else every 64th word.
+    // neighbours each where those are 16-byte loads, else every 64th word.  The conversions to 64 bits are what it costs: over a
+    // proposal some 90 cycles for 64 words, so a CU takes 128000 words in 20 us.
     template <bool Q>
     __device__ __forceinline__ double walk(int64_t from, int64_t to, int lane) const {
         constexpr int K = sizeof(E) == 4 ? 2 : 4;       // (sixteen waves leave 128 registers each)
@@ -50,12 +53,12 @@ struct Weights {
                 }
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-                    const int64_t c = c0 + 512 * k + 8 * lane;
+                    const int here = c0 + 512 * k + 8 * lane < to ? 8 : 0;
                     float x[8], y[8];
-                    a[k].put(x, c < to ? 8 : 0);
-                    if (Q) b[k].put(y, c < to ? 8 : 0);
+                    a[k].put(x, here);
+                    if (Q) b[k].put(y, here);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum += of(x[j], Q ? y[j] : c + j == certain ? 1.f : 0.f);
+                    for (int j = 0; j < 8; ++j) sum += Q ? over(x[j], y[j]) : over(x[j]);
                 }
             } else {
 #pragma unroll
@@ -69,9 +72,8 @@ struct Weights {
                     }
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int64_t c = c0 + 512 * k + 64 * j + lane;
-                        const double w = of((float)a[j], Q ? (float)b[j] : c == certain ? 1.f : 0.f);
-                        sum += c < to ? w : 0.0;
+                        const double w = Q ? over((float)a[j], (float)b[j]) : over((float)a[j]);
+                        sum += c0 + 512 * k + 64 * j + lane < to ? w : 0.0;
                     }
                 }
             }
@@ -79,30 +81,25 @@ struct Weights {
         return sum;
     }
     __device__ __forceinline__ double sum(int64_t from, int64_t to, int lane) const {
-        return wave_sum64(q ? walk<true>(from, to, lane) : walk<false>(from, to, lane));
+        if (q) return wave_sum64(walk<true>(from, to, lane));
+        if (certain < from || certain >= to) return wave_sum64(walk<false>(from, to, lane));
+        // A certain proposal's word weighs p - 1 (0 unless p is over 1), not p.  Taken back from the sum it would leave a rounding behind,
+        // so the 512 words around it are summed without it.
+        const int64_t c0 = from + ((certain - from) & ~(int64_t)511), c1 = min(c0 + 512, to);
+        double s = walk<false>(from, c0, lane) + walk<false>(c1, to, lane);
+        for (int64_t c = c0 + lane; c < c1; c += 64) s += at(c);
+        return wave_sum64(s);
     }
 };
 
-// One workgroup of NW waves a caption.  The vocabulary is cut into NW stretches, a wave sums one; the stretch that the draw falls into is
-// cut again if it is long, and one wave walks the rest word by word.  That reads the rows once and a sixteenth (a 256th) of them again,
-// and no sum's order depends on anything but v, so results repeat.  Bound: at one caption the chain of dependent reads (draft ->
-// probabilities -> rows -> stretch), at many reading two rows each.
-template <OpType T, int NW, bool WIDE>
-__global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
-    typedef typename Elem<T>::type E;
-    __shared__ double part[2][2][NW];       // [turn][level]: never written again while a wave may still read it
-    const int64_t i = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t* drafts = a.draft + i * a.draft_b;
-    auto draft = [&](int j) { return drafts[j * a.draft_j]; };
-    // every wave finds the first refused word for itself, a lane a word
-    const int len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j;
-    int n = len;
+// The first word of caption i's draft that is refused, or its length; every wave finds it for itself, a lane a word.
+template <OpType T>
+__device__ __forceinline__ int first_refused(const VerifyArgs& a, int64_t i, int len, int lane) {
     for (int j0 = 0; j0 < len; j0 += 64) {
         const int j = j0 + lane;
         bool kept = true;
         if (j < len) {
-            const int64_t d = draft(j);
+            const int64_t d = a.draft[i * a.draft_b + j * a.draft_j];
             kept = d >= 0 && d < a.v;
             if (kept) {
                 const double p = prob<T>(a.target, i * a.target_b + j * a.target_j + d);
@@ -111,50 +108,111 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
             }
         }
         const unsigned long long refused = __ballot(!kept);
-        if (refused) { n = j0 + __builtin_ctzll(refused); break; }
+        if (refused) return __builtin_amdgcn_readfirstlane(j0 + __builtin_ctzll(refused));
     }
-    n = __builtin_amdgcn_readfirstlane(n);
+    return len;
+}
+template <OpType T, bool WIDE>
+__device__ __forceinline__ Weights<T, WIDE> weights_at(const VerifyArgs& a, int64_t i, int n, int len) {
+    typedef typename Elem<T>::type E;
     Weights<T, WIDE> w;
-    w.v = a.v;
     w.p = static_cast<const E*>(a.target) + i * a.target_b + n * a.target_j;
     w.q = n < len && a.proposal ? static_cast<const E*>(a.proposal) + i * a.proposal_b + n * a.proposal_j : nullptr;
-    w.certain = n < len && !a.proposal ? draft(n) : -1;
+    w.certain = n < len && !a.proposal ? a.draft[i * a.draft_b + n * a.draft_j] : -1;
+    return w;
+}
+// The vocabulary in `n` stretches: multiples of 512 words, as many as 64 lanes take at a time.
+__device__ __forceinline__ int64_t stretch(int64_t v, int n) { return ((v + n - 1) / n + 511) & ~(int64_t)511; }
+// Running sums of the stretches, four neighbours a lane (a loop over them, one dependent read and addition after the other, took longer
+// than reading the rows).
+struct Running {
+    double x[4], incl;              // this lane's stretches; the sum up to and with them
+    __device__ __forceinline__ Running(const double* all, int n, int lane) {
+        double own = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[j] = 4 * lane + j < n ? all[4 * lane + j] : 0.0; own += x[j]; }
+        incl = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const double y = __shfl_up(incl, o, 64); if (lane >= o) incl += y; }
+    }
+    __device__ __forceinline__ double total() const { return __shfl(incl, 63, 64); }
+    // The stretch in which the running sum from `base` on passes t, and (in `base`) the sum in front of it; where roundings leave none,
+    // the last with any weight.
+    __device__ __forceinline__ int passes(double t, double& base, int lane) const {
+        int first = -1, some = -1;
+        double run = base + (incl - ((x[0] + x[1]) + (x[2] + x[3]))), at_first = 0.0, at_some = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double next = run + x[j];
+            if (x[j] > 0.0) {
+                some = 4 * lane + j; at_some = run;
+                if (next > t && first < 0) { first = 4 * lane + j; at_first = run; }
+            }
+            run = next;
+        }
+        const unsigned long long over = __ballot(first >= 0), with = __ballot(some >= 0);
+        const int from = over ? __builtin_ctzll(over) : with ? 63 - __builtin_clzll(with) : 0;
+        base = __shfl(over ? at_first : at_some, from, 64);
+        return __builtin_amdgcn_readfirstlane(__shfl(over ? first : some, from, 64));
+    }
+};
+
+constexpr int NW16 = 16;
+
+// The stretches' sums of long rows by several workgroups a caption (blockIdx.x of gridDim.x), for verify_kernel to go on from.
+template <OpType T, bool WIDE>
+__global__ __launch_bounds__(64 * NW16) void verify_sums_kernel(VerifyArgs a) {
+    const int64_t i = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ns = gridDim.x * NW16, k = blockIdx.x * NW16 + wave;
+    const int len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j, n = first_refused<T>(a, i, len, lane);
+    const Weights<T, WIDE> w = weights_at<T, WIDE>(a, i, n, len);
+    const int64_t step = stretch(a.v, ns), lo = min(k * step, a.v), hi = min(lo + step, a.v);
+    const double mine = lo < hi ? w.sum(lo, hi, lane) : 0.0;
+    if (lane == 0) a.sums[i * ns + k] = mine;
+}
+
+// One workgroup of NW waves a caption.  The vocabulary is cut into NW stretches, a wave sums one (or the sums of `split` * 16 stretches are
+// there already); the stretch that the draw falls into is cut again if it is long, and one wave walks the rest word by word.  That reads
+// the rows once and a sixteenth (a 256th) of them again, and no sum's order depends on anything but v and b, so results repeat.  Bound: at
+// one caption the chain of dependent reads (draft -> probabilities -> rows -> stretch), at many reading two rows each.
+template <OpType T, int NW, bool WIDE>
+__global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
+    __shared__ double given[VERIFY_SPLIT * NW16];
+    __shared__ double part[2][2][NW];       // [turn][level]: never written again while a wave may still read it
+    const int64_t i = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j, n = first_refused<T>(a, i, len, lane);
+    Weights<T, WIDE> w = weights_at<T, WIDE>(a, i, n, len);
     const double u = (double)a.draw_u[i];
 
     int64_t word = -1;
     for (int turn = 0; turn < 2; ++turn) {
-        // a stretch of the vocabulary for each wave: multiples of 512 words, as many as 64 lanes take at a time
-        int64_t from = 0, to = a.v, step = ((a.v + NW - 1) / NW + 511) & ~(int64_t)511;
+        const bool there = turn == 0 && a.split > 1;
+        const int ns = there ? a.split * NW16 : NW;
+        int64_t from = 0, to = a.v, step = stretch(a.v, ns);
         double base = 0.0, t = 0.0;
         bool any = false;
         for (int level = 0; level < 2; ++level) {
-            const int64_t lo = min(from + wave * step, to), hi = min(lo + step, to);
-            const double mine = lo < hi ? w.sum(lo, hi, lane) : 0.0;
-            if (lane == 0) part[turn][level][wave] = mine;
+            if (level == 0 && there) {
+                for (int k = tid; k < ns; k += 64 * NW) given[k] = a.sums[i * ns + k];
+            } else {
+                const int64_t lo = min(from + wave * step, to), hi = min(lo + step, to);
+                const double mine = lo < hi ? w.sum(lo, hi, lane) : 0.0;
+                if (lane == 0) part[turn][level][wave] = mine;
+            }
             __syncthreads();
-            const double* all = part[turn][level];
+            const double* all = level == 0 && there ? given : part[turn][level];
+            const Running run(all, level == 0 ? ns : NW, lane);
             if (level == 0) {
-                double total = 0.0;
-                for (int k = 0; k < NW; ++k) total += all[k];
+                const double total = run.total();
                 any = total > 0.0;
                 if (!any) break;
                 t = u * total;
             }
-            // the stretch in which the running sum passes t; where roundings leave none, the last with any weight
-            int hit = -1, last = 0;
-            double before = base, c = base;
-            for (int k = 0; k < NW; ++k) {
-                if (all[k] > 0.0 && hit < 0) {
-                    last = k; before = c;
-                    if (c + all[k] > t) hit = k;
-                }
-                c += all[k];
-            }
-            base = before;
-            from = min(from + last * step, to);
+            from = min(from + max(run.passes(t, base, lane), 0) * step, to);
             to = min(from + step, to);
             if (step <= 2048) break;
-            step = ((to - from + NW - 1) / NW + 511) & ~(int64_t)511;
+            step = stretch(to - from, NW);
         }
         if (any) {
             if (wave == 0) {                 // word by word: eight neighbours a lane, 512 at a time
@@ -185,22 +243,25 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
         w.q = nullptr; w.certain = -1;       // nothing is left over a proposal that is nowhere smaller: the draw is from p itself
     }
     if (wave == 0)
-        for (int k = lane; k <= a.j; k += 64) a.words[i * a.words_ld + k] = k < n ? draft(k) : k == n ? word : -1;
+        for (int k = lane; k <= a.j; k += 64) a.words[i * a.words_ld + k] = k < n ? a.draft[i * a.draft_b + k * a.draft_j] : k == n ? word : -1;
     if (tid == 0) a.accepted[i] = n;
 }
 
-template <OpType T, int NW>
+template <OpType T, bool WIDE>
 static hipError_t run(hipStream_t s, const VerifyArgs& a) {
-    constexpr size_t size = sizeof(typename Elem<T>::type);
-    const bool wide = eights_are_wide(a.target, a.target_b, a.v, size) && a.target_j * (int64_t)size % 16 == 0 &&
-                      (!a.proposal || (eights_are_wide(a.proposal, a.proposal_b, a.v, size) && a.proposal_j * (int64_t)size % 16 == 0));
-    if (wide) verify_kernel<T, NW, true><<<dim3((unsigned)a.b), 64 * NW, 0, s>>>(a);
-    else verify_kernel<T, NW, false><<<dim3((unsigned)a.b), 64 * NW, 0, s>>>(a);
+    if (a.split > 1) verify_sums_kernel<T, WIDE><<<dim3((unsigned)a.split, (unsigned)a.b), 64 * NW16, 0, s>>>(a);
+    if (a.v <= 4 * 512) verify_kernel<T, 4, WIDE><<<dim3((unsigned)a.b), 64 * 4, 0, s>>>(a);
+    else verify_kernel<T, NW16, WIDE><<<dim3((unsigned)a.b), 64 * NW16, 0, s>>>(a);
     return hipGetLastError();
 }
 
 template <OpType T>
-static hipError_t run(hipStream_t s, const VerifyArgs& a) { return a.v <= 4 * 512 ? run<T, 4>(s, a) : run<T, 16>(s, a); }
+static hipError_t run(hipStream_t s, const VerifyArgs& a) {
+    constexpr size_t size = sizeof(typename Elem<T>::type);
+    const bool wide = eights_are_wide(a.target, a.target_b, a.v, size) && a.target_j * (int64_t)size % 16 == 0 &&
+                      (!a.proposal || (eights_are_wide(a.proposal, a.proposal_b, a.v, size) && a.proposal_j * (int64_t)size % 16 == 0));
+    return wide ? run<T, true>(s, a) : run<T, false>(s, a);
+}
 
 hipError_t launch_verify_draft(hipStream_t s, const VerifyArgs& a) {
     return a.type == OP_F32 ? run<OP_F32>(s, a) : a.type == OP_BF16 ? run<OP_BF16>(s, a) : run<OP_F16>(s, a);

@@ -228,9 +228,11 @@ def verify_draft(draft, target, proposal, accept_u, draw_u, lens=None):
     device = target.device
     words = _empty((b, j + 1), dtype=_I64, device=device)
     accepted = _empty((b,), dtype=_I32, device=device)
-    rc = _native.load_library().stattn_verify_draft(dev, _raw_stream(dev), draft.data_ptr(), db, target.data_ptr(), tb, tj, pp, pb, pj, dtype,
-                                                    accept_u.data_ptr(), ub, draw_u.data_ptr(), pl, b, j, v, words.data_ptr(), j + 1,
-                                                    accepted.data_ptr())
+    lib = _native.load_library()
+    need = lib.stattn_verify_draft_workspace(b, j, v)
+    work = _empty((need,), dtype=_U8, device=device) if need else None        # alive until the launches are enqueued
+    rc = lib.stattn_verify_draft(dev, _raw_stream(dev), draft.data_ptr(), db, target.data_ptr(), tb, tj, pp, pb, pj, dtype, accept_u.data_ptr(), ub,
+                                 draw_u.data_ptr(), pl, b, j, v, words.data_ptr(), j + 1, accepted.data_ptr(), work.data_ptr() if need else None, need)
     if rc:
         _fail(rc)
     return words, accepted
