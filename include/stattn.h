@@ -172,7 +172,7 @@ int stattn_sample_search(stattn_handle* h, int nvid, const float* ctxg, const fl
  * `draft` words (1 .. 8) one after the other on the decoder's own states, then ONE product with the full-precision matrix gives the
  * distributions in front of all of them and behind the last, and stattn_verify_draft keeps as many drafts as make the caption a
  * sample of those, plus one word drawn from them.  Between 1 and draft + 1 words a round, whatever the 4-bit copy is worth.
- * 1 <= nvid <= 16; features as in stattn_sample_search; every precision.  `uniforms`: the numbers in [0, 1) that decide, host memory
+ * 1 <= nvid <= 16, 1 <= maxlen <= 65536; features as in stattn_sample_search; every precision.  `uniforms`: the numbers in [0, 1) that decide, host memory
  * (maxlen, 2 * draft + 1, nvid) -- a round takes one row each for the draws of its drafts, for their checks and for the last word --
  * or NULL: from the handle's seed and a per-call counter.  out_drafted / out_kept (nvid) or NULL: words drafted and kept, a caption. */
 int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl,
@@ -286,7 +286,7 @@ int stattn_allreduce_scalars(stattn_handle* h, float* vals, int n);
  *   codes  (rows, kp / 2) bytes, two columns a byte, the even one in the low half: sign, 2 bits of exponent, 1 of mantissa
  *          (0, 0.5, 1, 1.5, 2, 3, 4, 6);
  *   scales (rows, kp / 32) bytes: byte s of a block of 32 columns multiplies its codes by 2^(s - 127); 255 makes the block NaN.
- * Both 16-byte aligned.  Columns behind the last one hold code 0 (they must, when the form comes from elsewhere and is multiplied). */
+ * Codes 16-byte, scales 4-byte aligned, so any run of rows is such a matrix too.  Columns behind the last one hold code 0 (they must, when the form comes from elsewhere and is multiplied). */
 #define STATTN_F32 0
 #define STATTN_BF16 1
 #define STATTN_F16 2

@@ -120,9 +120,11 @@ def check_product(y, a, w, bias, k, out):
     assert y.dtype == out and (err <= tol).all(), (err - tol).max()
 
 
+# (the last four: 128 x 128 tiles, twice, and 256 x 256 tiles; the last stage of 256 columns is half there in the first and third)
 SHAPES = [(1, 1, 1), (1, 33, 128), (2, 16, 31), (5, 100, 129), (16, 64, 256), (17, 129, 511), (31, 255, 640), (33, 32, 1024), (64, 700, 96),
           (65, 66, 2050), (129, 257, 300), (255, 300, 1300), (257, 513, 257), (300, 40, 4096), (1, 5000, 513), (700, 1, 384), (12, 12, 12000),
-          (513, 2049, 128), (1000, 1300, 160), (260, 2100, 4100)]
+          (513, 2049, 128), (1000, 1300, 160), (260, 2100, 4100),
+          (2100, 2100, 300), (2050, 2300, 700), (3000, 2900, 1030), (2950, 3100, 1200)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
@@ -173,6 +175,33 @@ def test_linear_of_strided_rows_and_odd_addresses(ops):
             assert torch.equal(ops.mx4_linear(v, qw), ops.mx4_linear(v.contiguous(), qw))
         with pytest.raises(ValueError):
             ops.mx4_linear(base[:, ::3][:, :200], qw)
+
+
+@pytest.mark.parametrize("k", [100, 300, 640])
+def test_a_run_of_rows_is_a_matrix_too(ops, k):
+    """Rows 7 .. 64 of a form, whose scales start at any multiple of four bytes."""
+    q, x = ops.mx4_quantize(torch.randn(90, k, device=DEV)), torch.randn(33, k, device=DEV)
+    part = ops.MX4(q.codes[7:64], q.scales[7:64], k)
+    assert torch.equal(ops.mx4_dequantize(part), ops.mx4_dequantize(q)[7:64])
+    assert torch.equal(ops.mx4_linear(x, part), ops.mx4_linear(x, q)[:, 7:64])
+    assert torch.equal(ops.mx4_matmul(part, q), ops.mx4_matmul(q, q)[7:64])
+    assert torch.equal(ops.mx4_matmul(q, part), ops.mx4_matmul(q, q)[:, 7:64])
+
+
+def test_rows_behind_the_last_and_columns_beside_are_left_alone(ops):
+    """Through the C entry: y inside a larger buffer, every tile size, both types of store; nothing beside it is touched."""
+    from stattn import _native
+    lib = _native.load_library()
+    for m, n, k, dtype, code in [(5, 33, 64, torch.float32, 0), (70, 130, 300, torch.bfloat16, 1), (1100, 1000, 256, torch.float16, 2), (2100, 3900, 1200, torch.bfloat16, 1)]:
+        a, w = ops.mx4_quantize(torch.randn(m, k, device=DEV)), ops.mx4_quantize(torch.randn(n, k, device=DEV))
+        big = torch.full((m + 5, n + 37), 7.0, dtype=dtype, device=DEV)
+        y = big[2:2 + m, 3:3 + n]
+        rc = lib.stattn_mx4_matmul(0, torch.cuda.current_stream().cuda_stream, a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
+                                   m, n, k, None, y.data_ptr(), code, n + 37)
+        assert rc == 0
+        assert torch.equal(y, ops.mx4_matmul(a, w, dtype=dtype))
+        big[2:2 + m, 3:3 + n] = 7.0
+        assert bool((big == 7.0).all())
 
 
 def test_no_rows_no_outputs(ops):

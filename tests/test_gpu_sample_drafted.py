@@ -179,7 +179,7 @@ def test_refusals(stattn_mod, O):
     with pytest.raises(ValueError, match="nvid"):
         dec.sample_drafted(*features(b))
     two = features(b, slice(0, 2))
-    for kw in (dict(draft=0), dict(draft=9), dict(maxlen=0)):
+    for kw in (dict(draft=0), dict(draft=9), dict(maxlen=0), dict(maxlen=65537)):
         with pytest.raises(ValueError):
             dec.sample_drafted(*two, **kw)
     with pytest.raises(ValueError):

@@ -53,7 +53,8 @@ def test_matmul_and_linear_refusals():
     refused(f(0, None, A, A, A, A, 4, 8, 32, None, A, 0, 1 << 22), "ld_y")
     refused(f(0, None, A, A, A, A, 4, 8, 32, None, A, 9, 8), "dtype")
     refused(f(0, None, A, A, A, A, 4, 8, 32, None, None, 0, 8), "null y")
-    refused(f(0, None, A, A, A, A + 4, 4, 8, 32, None, A, 0, 8), "aligned")
+    refused(f(0, None, A, A, A, A + 2, 4, 8, 32, None, A, 0, 8), "aligned")
+    refused(f(0, None, A, A, A + 8, A, 4, 8, 32, None, A, 0, 8), "aligned")
     refused(f(0, None, A, A, A, A, 1 << 20, 1 << 20, 32, None, A, 0, 1 << 20), "too large")
     refused(f(0, None, None, A, A, A, 4, 8, 32, None, A, 0, 8), "null")
     assert f(0, None, None, None, A, A, 0, 8, 32, None, None, 0, 8) == 0

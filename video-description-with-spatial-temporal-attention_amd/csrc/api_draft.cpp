@@ -15,8 +15,8 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
                           int32_t* out_drafted, int32_t* out_kept) {
     const bool resident = !ctxg && !ctxg_mask && !ctxl && !ctxm;
     if (!h || nvid < 1 || nvid > 16 || (!resident && (!ctxg || !ctxg_mask || !ctxl || !ctxm)) || T <= 0 || K <= 0 || draft < 1 || draft > 8 ||
-        maxlen < 1 || !out_tokens || !out_scores || !out_lens)
-        return fail(h, STATTN_EINVAL, "sample_drafted: bad argument (1 <= nvid <= 16, 1 <= draft <= 8, maxlen >= 1)");
+        maxlen < 1 || maxlen > 65536 || !out_tokens || !out_scores || !out_lens)
+        return fail(h, STATTN_EINVAL, "sample_drafted: bad argument (1 <= nvid <= 16, 1 <= draft <= 8, 1 <= maxlen <= 65536)");
     HIPCHK(h, hipSetDevice(h->device));
     if (!resident) CHK(stattn_beam_stage(h, nvid, ctxg, ctxg_mask, ctxl, ctxm, T, K));
     else if (!h->bk_valid || h->bk_n != nvid || h->bk_T != T || h->bk_K != K)

@@ -41,7 +41,7 @@ int form_ok(const char* who, const void* codes, const void* scales, int64_t rows
     if (rows < 0 || rows >= MAX_ROWS || cols < 1 || cols > MAX_COLS)
         return refuse(STATTN_EINVAL, "%s: a matrix of %lld x %lld is outside 0 .. 2^31 - 1 rows and 1 .. 2^24 columns", who, (long long)rows, (long long)cols);
     if (rows && (!codes || !scales)) return refuse(STATTN_EINVAL, "%s: null codes or scales", who);
-    if (!al16(codes) || !al16(scales)) return refuse(STATTN_EINVAL, "%s: codes and scales must be 16-byte aligned", who);
+    if (!al16(codes) || (reinterpret_cast<uintptr_t>(scales) & 3)) return refuse(STATTN_EINVAL, "%s: codes must be 16-byte aligned, scales 4-byte aligned", who);
     return STATTN_OK;
 }
 
@@ -107,9 +107,10 @@ int stattn_mx4_matmul(int device, void* stream, const void* a_codes, const void*
 }
 
 // Few rows: one launch in which every workgroup rounds x for itself, instead of two with x's 4-bit form between them.  Up to 32768
-// values of x that is as fast on the GPU (1 x 12000 x 512: 3.9 us against 5.1; 16 x 20000 x 1024: 8.1 against 6.9; 64 x 20000 x 1024,
-// beyond: 18.7 against 7.4) and saves the caller a launch and a workspace, 5 us of its time.
-static bool few_rows(int64_t m, int64_t k) { return m <= 64 && m * k <= 32768; }
+// values of x that takes the GPU little longer (1 x 12000 x 512: 3.8 us against 5.1; 32: 6.0 against 5.6; 64: 8.9 against 5.8; beyond,
+// 64 x 20000 x 1024: 18.5 against 7.4) and saves the caller a launch and a workspace, 4.5 us of its time.  Rows whose last eight are
+// partial load one by one in between (64 x 12000 x 511: 12): up to 16384.
+static bool few_rows(int64_t m, int64_t k) { return m <= 64 && m * k <= (k % 8 ? 16384 : 32768); }
 
 size_t stattn_mx4_linear_workspace(int64_t m, int64_t n, int64_t k) {
     (void)n;

@@ -7,16 +7,16 @@ namespace stattn {
 // x row-major.  A lane takes eight columns (one or two 16-byte loads) and writes the word of their codes, so a wave reads and writes
 // whole lines; the four lanes of a block find its scale by two moves inside the quad.  (A lane per block, 32 columns each, read lines in
 // eight or four pieces: the regions of a batch, 13312 x 4096 bf16, took 125 us instead of XX.)
-template <OpType T, bool WIDE>
+template <OpType T>
 __global__ __launch_bounds__(256) void mx4_quantize_rows_kernel(Mx4QuantArgs a, unsigned words, int64_t n) {
     typedef typename Elem<T>::type E;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {      // n and the steps are multiples of 4
         const int64_t r = n >> 32 ? i / words : (int64_t)((unsigned)i / words);
-        const int c = (int)(i - r * words) * 8, here = (int)max(min(a.cols - c, (int64_t)8), (int64_t)0);
-        Eight<T, WIDE> x;
+        const int c = (int)(i - r * words) * 8;
+        Eight<T> x;
         float v[8];
-        x.take(static_cast<const E*>(a.x) + r * a.row_stride, c, here);
-        x.put(v, here);
+        x.take(static_cast<const E*>(a.x) + r * a.row_stride + c, (int)(a.cols - c));
+        x.put(v);
         const unsigned byte = mx4_scale_byte(quad_max(top8(v)));
         reinterpret_cast<unsigned*>(a.codes)[i] = mx4_codes8(v, byte);
         if ((threadIdx.x & 3) == 0) a.scales[i >> 2] = (uint8_t)byte;
@@ -65,10 +65,7 @@ static hipError_t quantize(hipStream_t s, const Mx4QuantArgs& a) {
     const int64_t kp = mx4_kp(a.cols);
     if (a.col_stride == 1 || a.cols == 1) {
         const int64_t n = a.rows * (kp / 8);
-        const bool wide = eights_are_wide(a.x, a.row_stride, a.cols, sizeof(typename Elem<T>::type));
-        const dim3 grid((unsigned)std::min((n + 255) / 256, FULL));
-        if (wide) mx4_quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(a, (unsigned)(kp / 8), n);
-        else mx4_quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(a, (unsigned)(kp / 8), n);
+        mx4_quantize_rows_kernel<T><<<dim3((unsigned)std::min((n + 255) / 256, FULL)), 256, 0, s>>>(a, (unsigned)(kp / 8), n);
     } else {
         const int64_t rt = (a.rows + 63) / 64;
         mx4_quantize_cols_kernel<T><<<dim3((unsigned)std::min(rt * (kp / 128), FULL)), 256, 0, s>>>(a, (unsigned)rt, (unsigned)(kp / 128));
@@ -83,9 +80,9 @@ hipError_t launch_mx4_quantize(hipStream_t s, const Mx4QuantArgs& a) {
 // A lane per eight columns: a word of codes, the block's scale, one or two 16-byte stores.  The code is turned into its number first and
 // multiplied by the scale after, so that the smallest scales (2^-127 is subnormal) and NaN need no case of their own.
 template <OpType T>
-__global__ __launch_bounds__(256) void mx4_dequantize_kernel(Mx4View q, typename Elem<T>::type* out, int64_t ld, unsigned words, int64_t n, bool wide) {
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(Mx4View q, typename Elem<T>::type* out, int64_t ld, unsigned words, int64_t n) {
     typedef typename Elem<T>::type E;
-    typedef E e8 __attribute__((ext_vector_type(8)));
+    typedef E e8 __attribute__((ext_vector_type(8), aligned(sizeof(E))));       // (16-byte stores to any element's address)
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t r = n >> 32 ? i / words : (int64_t)((unsigned)i / words);
         const int c = (int)(i - r * words) * 8;
@@ -99,7 +96,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(Mx4View q, typename
         put(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2));
         put(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3));
         E* o = out + r * ld + c;
-        if (wide && c + 8 <= q.cols) {
+        if (c + 8 <= q.cols) {
             *reinterpret_cast<e8*>(o) = v;
         } else {
 #pragma unroll
@@ -113,8 +110,7 @@ template <OpType T>
 static hipError_t dequantize(hipStream_t s, const Mx4View& q, void* out, int64_t ld) {
     typedef typename Elem<T>::type E;
     const int64_t words = mx4_kp(q.cols) / 8, n = q.rows * words;
-    const bool wide = (reinterpret_cast<uintptr_t>(out) & (sizeof(E) * 8 - 1)) == 0 && ld % 8 == 0;
-    mx4_dequantize_kernel<T><<<dim3((unsigned)std::min((n + 255) / 256, FULL)), 256, 0, s>>>(q, static_cast<E*>(out), ld, (unsigned)words, n, wide);
+    mx4_dequantize_kernel<T><<<dim3((unsigned)std::min((n + 255) / 256, FULL)), 256, 0, s>>>(q, static_cast<E*>(out), ld, (unsigned)words, n);
     return hipGetLastError();
 }
 

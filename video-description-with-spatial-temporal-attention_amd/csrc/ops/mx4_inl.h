@@ -50,30 +50,26 @@ __device__ __forceinline__ unsigned top8(const float* v) {
     return t;
 }
 // Eight neighbouring elements as they lie in memory: `take` requests them and `put` turns them into floats, so that a caller can have
-// several requests on their way.  Elements from number n (0 .. 8) on are not there and become 0.  WIDE: x is 16-byte aligned and n is
-// 0 or 8, one or two 16-byte loads without a branch (from the row's start where nothing is there); else element by element.
-template <OpType T, bool WIDE>
+// several requests on their way.  Elements from number n on are not there and become 0.  Any address will do: 16-byte loads need no more
+// than an element's alignment here (a row of odd length costs what an even one does); only a row's last, partial eight go one by one.
+template <OpType T>
 struct Eight {
     typedef typename Elem<T>::type E;
-    typedef E vec __attribute__((ext_vector_type(16 / sizeof(E))));
-    vec raw[WIDE ? sizeof(E) / 2 : 1];
-    E one[WIDE ? 1 : 8];
-    __device__ __forceinline__ void take(const E* row, int64_t c, int n) {
-        if constexpr (WIDE) {
-            const vec* x = reinterpret_cast<const vec*>(row + (n > 0 ? c : 0));
+    typedef E vec __attribute__((ext_vector_type(16 / sizeof(E)), aligned(sizeof(E))));
+    static constexpr int PARTS = sizeof(E) / 2, PER = 16 / sizeof(E);
+    vec raw[PARTS];
+    __device__ __forceinline__ void take(const E* x, int n) {
+        if (n >= 8) {
 #pragma unroll
-            for (int j = 0; j < (int)sizeof(E) / 2; ++j) raw[j] = x[j];
+            for (int j = 0; j < PARTS; ++j) raw[j] = reinterpret_cast<const vec*>(x)[j];
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) one[j] = row[j < n ? c + j : 0];
+            for (int j = 0; j < 8; ++j) raw[j / PER][j % PER] = j < n ? x[j] : (E)0.f;
         }
     }
-    __device__ __forceinline__ void put(float* v, int n) const {
+    __device__ __forceinline__ void put(float* v) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (WIDE) v[j] = n > 0 ? (float)raw[j / (16 / sizeof(E))][j % (16 / sizeof(E))] : 0.f;
-            else v[j] = j < n ? (float)one[j] : 0.f;
-        }
+        for (int j = 0; j < 8; ++j) v[j] = (float)raw[j / PER][j % PER];
     }
 };
 // the fp32 value of a scale byte (0 is 2^-127, a subnormal; 255 is NaN)

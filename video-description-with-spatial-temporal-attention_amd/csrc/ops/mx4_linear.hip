@@ -13,7 +13,7 @@ namespace stattn {
 // add up through LDS: for heads with few rows, where a wave a group would leave most of the chip without one.
 constexpr int U = 8;
 
-template <OpType T, int MT, int KS, bool WIDE>
+template <OpType T, int MT, int KS>
 __global__ __launch_bounds__(256) void mx4_linear_kernel(Mx4LinearArgs p) {
     typedef typename Elem<T>::type E;
     constexpr int BM = 16 * MT, KC = 4096 / MT;                      // 32 KB of codes
@@ -54,21 +54,20 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(Mx4LinearArgs p) {
         auto round_x = [&](auto requests) {                         // that many requests of a lane on their way
             constexpr int Q = decltype(requests)::value;
             for (int i0 = tid; i0 - tid < total; i0 += 256 * Q) {
-                Eight<T, WIDE> x[Q];
-                int at[Q], row[Q], here[Q];
+                Eight<T> x[Q];
+                int at[Q], row[Q];
 #pragma unroll
                 for (int q = 0; q < Q; ++q) {                       // (behind the end: the last words once more)
                     const int i = min(i0 + 256 * q, total - 4 + (tid & 3));
                     row[q] = (unsigned)i / (unsigned)words;
                     at[q] = i - row[q] * words;
                     const int64_t c = (int64_t)c0 * 128 + at[q] * 8;
-                    here[q] = (int)max(min(p.w.cols - c, (int64_t)8), (int64_t)0);
-                    x[q].take(static_cast<const E*>(p.x) + (m0 + row[q]) * p.ldx, c, here[q]);
+                    x[q].take(static_cast<const E*>(p.x) + (m0 + row[q]) * p.ldx + c, (int)(p.w.cols - c));
                 }
 #pragma unroll
                 for (int q = 0; q < Q; ++q) {
                     float v[8];
-                    x[q].put(v, here[q]);
+                    x[q].put(v);
                     const unsigned byte = mx4_scale_byte(quad_max(top8(v)));
                     *reinterpret_cast<unsigned*>(xc + row[q] * RS + at[q] * 4) = mx4_codes8(v, byte);
                     if ((at[q] & 3) == 0) xs[row[q] * SS + (at[q] >> 2)] = (uint8_t)byte;
@@ -131,18 +130,12 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(Mx4LinearArgs p) {
         }
 }
 
-template <OpType T, int MT, int KS>
-static hipError_t run(hipStream_t s, const Mx4LinearArgs& a, dim3 grid) {
-    if (eights_are_wide(a.x, a.ldx, a.w.cols, sizeof(typename Elem<T>::type))) mx4_linear_kernel<T, MT, KS, true><<<grid, 256, 0, s>>>(a);
-    else mx4_linear_kernel<T, MT, KS, false><<<grid, 256, 0, s>>>(a);
-    return hipGetLastError();
-}
-
 template <OpType T, int MT>
 static hipError_t run(hipStream_t s, const Mx4LinearArgs& a) {
     const unsigned gm = (unsigned)((a.m + 16 * MT - 1) / (16 * MT)), gn = (unsigned)((a.w.rows + 15) / 16);
-    if ((int64_t)gm * gn < 4 * 128 && a.w.cols > 128) return run<T, MT, 4>(s, a, dim3(gn, gm));
-    return run<T, MT, 1>(s, a, dim3((gn + 3) / 4, gm));
+    if ((int64_t)gm * gn < 4 * 128 && a.w.cols > 128) mx4_linear_kernel<T, MT, 4><<<dim3(gn, gm), 256, 0, s>>>(a);
+    else mx4_linear_kernel<T, MT, 1><<<dim3((gn + 3) / 4, gm), 256, 0, s>>>(a);
+    return hipGetLastError();
 }
 
 template <OpType T>

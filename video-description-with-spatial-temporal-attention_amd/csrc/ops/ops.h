@@ -14,11 +14,6 @@ enum OpType { OP_F32 = 0, OP_BF16 = 1, OP_F16 = 2 };
 struct Mx4View { const uint8_t* codes; const uint8_t* scales; int64_t rows; int64_t cols; };
 __host__ __device__ inline int64_t mx4_kp(int64_t cols) { return (cols + 127) / 128 * 128; }
 
-// whether every eight columns of a row-major matrix are one or two aligned 16-byte loads
-inline bool eights_are_wide(const void* x, int64_t ld, int64_t cols, size_t size) {
-    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * (int64_t)size % 16 == 0 && cols % 8 == 0;
-}
-
 struct Mx4QuantArgs {
     const void* x; OpType type; int64_t rows, cols, row_stride, col_stride;      // element (r, c) at x[r * row_stride + c * col_stride]
     uint8_t* codes; uint8_t* scales;

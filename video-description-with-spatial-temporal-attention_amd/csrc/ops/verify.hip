@@ -20,7 +20,7 @@ __device__ __forceinline__ double wave_sum64(double v) {
 
 // One caption's weights over a stretch of the vocabulary: p alone, p without the one word that a certain proposal has all its mass on, or
 // p over q.
-template <OpType T, bool WIDE>
+template <OpType T>
 struct Weights {
     typedef typename Elem<T>::type E;
     const E* p;
@@ -36,46 +36,28 @@ struct Weights {
     __device__ __forceinline__ double at(int64_t i) const { return q ? over((float)p[i], (float)q[i]) : i == certain ? over((float)p[i], 1.f) : over((float)p[i]); }
 
     // Sum of the weights from `from` to `to`, this lane's share of the wave's walk; K requests on their way.  The lanes take eight
-    // neighbours each where those are 16-byte loads, else every 64th word.  The conversions to 64 bits are what it costs: over a
+    // neighbours each.  The conversions to 64 bits are what it costs: over a
     // proposal some 90 cycles for 64 words, so a CU takes 128000 words in 20 us.
     template <bool Q>
     __device__ __forceinline__ double walk(int64_t from, int64_t to, int lane) const {
         constexpr int K = sizeof(E) == 4 ? 2 : 4;       // (sixteen waves leave 128 registers each)
         double sum = 0.0;
         for (int64_t c0 = from; c0 < to; c0 += 512 * K) {
-            if constexpr (WIDE) {
-                Eight<T, true> a[K], b[K];
+            Eight<T> a[K], b[K];
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    const int64_t c = c0 + 512 * k + 8 * lane;
-                    a[k].take(p, c, c < to ? 8 : 0);
-                    if (Q) b[k].take(q, c, c < to ? 8 : 0);
-                }
+            for (int k = 0; k < K; ++k) {
+                const int64_t c = c0 + 512 * k + 8 * lane;
+                const int here = (int)min(to - c, (int64_t)8);
+                a[k].take(p + c, here);
+                if (Q) b[k].take(q + c, here);
+            }
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    const int here = c0 + 512 * k + 8 * lane < to ? 8 : 0;
-                    float x[8], y[8];
-                    a[k].put(x, here);
-                    if (Q) b[k].put(y, here);
+            for (int k = 0; k < K; ++k) {
+                float x[8], y[8];
+                a[k].put(x);
+                if (Q) b[k].put(y);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum += Q ? over(x[j], y[j]) : over(x[j]);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    E a[8], b[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int64_t c = c0 + 512 * k + 64 * j + lane;
-                        a[j] = p[c < to ? c : from];
-                        if (Q) b[j] = q[c < to ? c : from];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const double w = Q ? over((float)a[j], (float)b[j]) : over((float)a[j]);
-                        sum += c0 + 512 * k + 64 * j + lane < to ? w : 0.0;
-                    }
-                }
+                for (int j = 0; j < 8; ++j) sum += Q ? over(x[j], y[j]) : over(x[j]);
             }
         }
         return sum;
@@ -112,10 +94,10 @@ __device__ __forceinline__ int first_refused(const VerifyArgs& a, int64_t i, int
     }
     return len;
 }
-template <OpType T, bool WIDE>
-__device__ __forceinline__ Weights<T, WIDE> weights_at(const VerifyArgs& a, int64_t i, int n, int len) {
+template <OpType T>
+__device__ __forceinline__ Weights<T> weights_at(const VerifyArgs& a, int64_t i, int n, int len) {
     typedef typename Elem<T>::type E;
-    Weights<T, WIDE> w;
+    Weights<T> w;
     w.p = static_cast<const E*>(a.target) + i * a.target_b + n * a.target_j;
     w.q = n < len && a.proposal ? static_cast<const E*>(a.proposal) + i * a.proposal_b + n * a.proposal_j : nullptr;
     w.certain = n < len && !a.proposal ? a.draft[i * a.draft_b + n * a.draft_j] : -1;
@@ -160,12 +142,12 @@ struct Running {
 constexpr int NW16 = 16;
 
 // The stretches' sums of long rows by several workgroups a caption (blockIdx.x of gridDim.x), for verify_kernel to go on from.
-template <OpType T, bool WIDE>
+template <OpType T>
 __global__ __launch_bounds__(64 * NW16) void verify_sums_kernel(VerifyArgs a) {
     const int64_t i = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ns = gridDim.x * NW16, k = blockIdx.x * NW16 + wave;
     const int len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j, n = first_refused<T>(a, i, len, lane);
-    const Weights<T, WIDE> w = weights_at<T, WIDE>(a, i, n, len);
+    const Weights<T> w = weights_at<T>(a, i, n, len);
     const int64_t step = stretch(a.v, ns), lo = min(k * step, a.v), hi = min(lo + step, a.v);
     const double mine = lo < hi ? w.sum(lo, hi, lane) : 0.0;
     if (lane == 0) a.sums[i * ns + k] = mine;
@@ -175,14 +157,14 @@ __global__ __launch_bounds__(64 * NW16) void verify_sums_kernel(VerifyArgs a) {
 // there already); the stretch that the draw falls into is cut again if it is long, and one wave walks the rest word by word.  That reads
 // the rows once and a sixteenth (a 256th) of them again, and no sum's order depends on anything but v and b, so results repeat.  Bound: at
 // one caption the chain of dependent reads (draft -> probabilities -> rows -> stretch), at many reading two rows each.
-template <OpType T, int NW, bool WIDE>
+template <OpType T, int NW>
 __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
     __shared__ double given[VERIFY_SPLIT * NW16];
     __shared__ double part[2][2][NW];       // [turn][level]: never written again while a wave may still read it
     const int64_t i = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j, n = first_refused<T>(a, i, len, lane);
-    Weights<T, WIDE> w = weights_at<T, WIDE>(a, i, n, len);
+    Weights<T> w = weights_at<T>(a, i, n, len);
     const double u = (double)a.draw_u[i];
 
     int64_t word = -1;
@@ -247,20 +229,12 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
     if (tid == 0) a.accepted[i] = n;
 }
 
-template <OpType T, bool WIDE>
-static hipError_t run(hipStream_t s, const VerifyArgs& a) {
-    if (a.split > 1) verify_sums_kernel<T, WIDE><<<dim3((unsigned)a.split, (unsigned)a.b), 64 * NW16, 0, s>>>(a);
-    if (a.v <= 4 * 512) verify_kernel<T, 4, WIDE><<<dim3((unsigned)a.b), 64 * 4, 0, s>>>(a);
-    else verify_kernel<T, NW16, WIDE><<<dim3((unsigned)a.b), 64 * NW16, 0, s>>>(a);
-    return hipGetLastError();
-}
-
 template <OpType T>
 static hipError_t run(hipStream_t s, const VerifyArgs& a) {
-    constexpr size_t size = sizeof(typename Elem<T>::type);
-    const bool wide = eights_are_wide(a.target, a.target_b, a.v, size) && a.target_j * (int64_t)size % 16 == 0 &&
-                      (!a.proposal || (eights_are_wide(a.proposal, a.proposal_b, a.v, size) && a.proposal_j * (int64_t)size % 16 == 0));
-    return wide ? run<T, true>(s, a) : run<T, false>(s, a);
+    if (a.split > 1) verify_sums_kernel<T><<<dim3((unsigned)a.split, (unsigned)a.b), 64 * NW16, 0, s>>>(a);
+    if (a.v <= 4 * 512) verify_kernel<T, 4><<<dim3((unsigned)a.b), 64 * 4, 0, s>>>(a);
+    else verify_kernel<T, NW16><<<dim3((unsigned)a.b), 64 * NW16, 0, s>>>(a);
+    return hipGetLastError();
 }
 
 hipError_t launch_verify_draft(hipStream_t s, const VerifyArgs& a) {
