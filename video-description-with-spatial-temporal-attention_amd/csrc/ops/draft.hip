@@ -105,9 +105,9 @@ hipError_t launch_softmax_draw(hipStream_t s, const DrawArgs& a) {
 }
 
 // A caption's share of the next round's uniform numbers: row r of a round holds one number a caption
-__device__ __forceinline__ void next_numbers(const DraftState& d, int m, int round) {
+__device__ __forceinline__ void next_numbers(const DraftState& d, int m, int round, int lane) {
     const int rows = 2 * d.k + 1;
-    for (int r = threadIdx.x; r < rows && round < d.maxlen; r += blockDim.x) d.u[r * d.M + m] = d.uniforms[((int64_t)round * rows + r) * d.M + m];
+    for (int r = lane; r < rows && round < d.maxlen; r += 64) d.u[r * d.M + m] = d.uniforms[((int64_t)round * rows + r) * d.M + m];
 }
 
 __global__ __launch_bounds__(256) void draft_begin_kernel(DraftState d, const float* h0, const float* c0) {
@@ -118,38 +118,44 @@ __global__ __launch_bounds__(256) void draft_begin_kernel(DraftState d, const fl
         d.x[m] = -1;
         d.info[m] = DraftInfo{0, 0, 0, 0, 0, 0.f};
     }
-    next_numbers(d, m, 0);
+    if (threadIdx.x < 64) next_numbers(d, m, 0, threadIdx.x);
 }
 
 // words row m: n = accepted[m] kept drafts, then the drawn word.  hs / cs (and projs, 8 D wide) hold the states behind each of the round's
 // k + 1 inputs (the last word, then the drafts), p the target's rows in front of each word.
-__global__ __launch_bounds__(256) void draft_commit_kernel(DraftState d, const int64_t* words, const int32_t* accepted, const float* hs, const float* cs,
-                                                           const float* projs, const float* p, int64_t ldp) {
-    const int m = blockIdx.x;
+__global__ __launch_bounds__(1024) void draft_commit_kernel(DraftState d, const int64_t* words, const int32_t* accepted, const float* hs, const float* cs,
+                                                            const float* projs, const float* p, int64_t ldp) {
+    const int m = blockIdx.x, t = threadIdx.x;
     DraftInfo f = d.info[m];
-    __syncthreads();                       // (thread 0 writes it below)
-    if (f.done) return;
     const int n = accepted[m];
-    const float* h = hs + ((int64_t)n * d.M + m) * d.D;
-    const float* c = cs + ((int64_t)n * d.M + m) * d.D;
-    for (int i = threadIdx.x; i < d.D; i += 256) { d.h[(int64_t)m * d.D + i] = h[i]; d.c[(int64_t)m * d.D + i] = c[i]; }
+    __syncthreads();                       // (the first wave writes it below)
+    if (f.done) return;
+    const int64_t from = (int64_t)n * d.M + m;
+    for (int i = t; i < d.D; i += 1024) { d.h[(int64_t)m * d.D + i] = hs[from * d.D + i]; d.c[(int64_t)m * d.D + i] = cs[from * d.D + i]; }
     if (projs)
-        for (int i = threadIdx.x; i < 8 * d.D; i += 256) d.proj[(int64_t)m * 8 * d.D + i] = projs[((int64_t)n * d.M + m) * 8 * d.D + i];
-    if (threadIdx.x == 0) {
-        f.drafted += d.k; f.kept += n;
-        int64_t w = 0;
-        for (int j = 0; j <= n && !f.done; ++j) {
-            w = words[(int64_t)m * (d.k + 1) + j];
-            if (w < 0) { f.done = 1; break; }                       // no word can be drawn (a model of NaNs): the caption ends here
-            d.tokens[(int64_t)m * d.maxlen + f.len++] = w;
-            f.score += p[((int64_t)j * d.M + m) * ldp + w];
-            f.done = w == 0 || f.len == d.maxlen;
-        }
-        d.x[m] = w < 0 ? 0 : w;
-        ++f.rounds;
+        for (int i = t; i < 2 * d.D; i += 1024)
+            reinterpret_cast<float4*>(d.proj)[(int64_t)m * 2 * d.D + i] = reinterpret_cast<const float4*>(projs)[from * 2 * d.D + i];
+    if (t < 64) next_numbers(d, m, f.rounds + 1, t);
+    if (t >= 64) return;
+    // one wave: lane j has word j of the round (at most 8 drafts and the drawn one) and its probability
+    const int64_t w = t <= n ? words[(int64_t)m * (d.k + 1) + t] : -1;
+    const float pw = w >= 0 ? p[((int64_t)t * d.M + m) * ldp + w] : 0.f;
+    // the caption takes words up to its first <eos>, its length's end, or the first that could not be drawn (a model of NaNs)
+    const unsigned long long ends = __ballot(t <= n && w <= 0), bad = __ballot(t <= n && w < 0);
+    const int stop = ends ? __builtin_ctzll(ends) : n;
+    int take = min(stop + 1, d.maxlen - f.len);
+    if (bad && __builtin_ctzll(bad) < take) take = __builtin_ctzll(bad);
+    if (t < take) d.tokens[(int64_t)m * d.maxlen + f.len + t] = w;
+    float score = f.score;
+    for (int j = 0; j < take; ++j) score += __shfl(pw, j, 64);
+    const int64_t last = __shfl(w, n, 64);
+    if (t == 0) {
+        f.drafted += d.k; f.kept += n; ++f.rounds;
+        f.len += take; f.score = score;
+        f.done = ends != 0 || f.len == d.maxlen;
+        d.x[m] = last < 0 ? 0 : last;
         d.info[m] = f;
     }
-    next_numbers(d, m, f.rounds + (threadIdx.x ? 1 : 0));          // thread 0 has counted the round already
 }
 
 hipError_t launch_draft_begin(hipStream_t s, const DraftState& d, const float* h0, const float* c0) {
@@ -158,7 +164,7 @@ hipError_t launch_draft_begin(hipStream_t s, const DraftState& d, const float* h
 }
 hipError_t launch_draft_commit(hipStream_t s, const DraftState& d, const int64_t* words, const int32_t* accepted, const float* hs, const float* cs,
                                const float* projs, const float* p, int64_t ldp) {
-    draft_commit_kernel<<<dim3((unsigned)d.M), 256, 0, s>>>(d, words, accepted, hs, cs, projs, p, ldp);
+    draft_commit_kernel<<<dim3((unsigned)d.M), 1024, 0, s>>>(d, words, accepted, hs, cs, projs, p, ldp);
     return hipGetLastError();
 }
 

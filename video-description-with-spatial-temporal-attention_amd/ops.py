@@ -18,7 +18,6 @@ except ImportError:
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
 _U8, _F32, _I32, _I64 = torch.uint8, torch.float32, torch.int32, torch.int64
-_empty = torch.empty
 # The checks below are written out, plain comparisons on the way of a good call: of the 7 us that a small product takes a caller, 3.5 are
 # the launch and 1.7 the result's allocation.
 
@@ -93,9 +92,8 @@ def mx4_quantize(x, axis=-1):
     if axis in (0, -2):
         rows, cols, rs, cs = cols, rows, cs, rs
     kb = (cols + 127) // 128 * 4
-    device = x.device
-    codes = _empty((rows, 16 * kb), dtype=_U8, device=device)
-    scales = _empty((rows, kb), dtype=_U8, device=device)
+    codes = x.new_empty((rows, 16 * kb), dtype=_U8)
+    scales = codes.new_empty((rows, kb))
     rc = _native.load_library().stattn_mx4_quantize(dev, _raw_stream(dev), x.data_ptr(), dtype, rows, cols, rs, cs, codes.data_ptr(), scales.data_ptr())
     if rc:
         _fail(rc)
@@ -112,7 +110,7 @@ def mx4_dequantize(q, dtype=torch.float32):
     if dev < 0 or scales.get_device() != dev:
         _wrong_place(dev, scales=scales)
     rows = codes.shape[0]
-    out = _empty((rows, cols), dtype=dtype, device=codes.device)
+    out = codes.new_empty((rows, cols), dtype=dtype)
     rc = _native.load_library().stattn_mx4_dequantize(dev, _raw_stream(dev), codes.data_ptr(), scales.data_ptr(), rows, cols, out.data_ptr(), t, cols)
     if rc:
         _fail(rc)
@@ -143,7 +141,7 @@ def mx4_matmul(a, w, bias=None, dtype=torch.float32):
         _wrong_place(dev, a_scales=as_, w=wc, w_scales=ws)
     m, n = ac.shape[0], wc.shape[0]
     b = None if bias is None else _check_bias(bias, n, dev)
-    y = _empty((m, n), dtype=dtype, device=ac.device)
+    y = ac.new_empty((m, n), dtype=dtype)
     rc = _native.load_library().stattn_mx4_matmul(dev, _raw_stream(dev), ac.data_ptr(), as_.data_ptr(), wc.data_ptr(), ws.data_ptr(), m, n, k, b,
                                                   y.data_ptr(), t, n)
     if rc:
@@ -173,10 +171,9 @@ def mx4_linear(x, w, bias=None):
     n = wc.shape[0]
     b = None if bias is None else _check_bias(bias, n, dev)
     lib = _native.load_library()
-    device = x.device
-    y = _empty((m, n), dtype=x.dtype, device=device)
+    y = x.new_empty((m, n))
     need = lib.stattn_mx4_linear_workspace(m, n, k)
-    work = _empty((need,), dtype=_U8, device=device) if need else None        # alive until the launches are enqueued
+    work = x.new_empty((need,), dtype=_U8) if need else None        # alive until the launches are enqueued
     rc = lib.stattn_mx4_linear(dev, _raw_stream(dev), x.data_ptr(), dtype, ld, wc.data_ptr(), ws.data_ptr(), m, n, k, b, y.data_ptr(), n,
                                work.data_ptr() if need else None, need)
     if rc:
@@ -225,12 +222,11 @@ def verify_draft(draft, target, proposal, accept_u, draw_u, lens=None):
         wrong = wrong or lens.get_device() != dev
     if wrong:
         _wrong_place(dev, draft=draft, proposal=proposal, accept_u=accept_u, draw_u=draw_u, lens=lens)
-    device = target.device
-    words = _empty((b, j + 1), dtype=_I64, device=device)
-    accepted = _empty((b,), dtype=_I32, device=device)
+    words = draft.new_empty((b, j + 1))
+    accepted = draft.new_empty((b,), dtype=_I32)
     lib = _native.load_library()
     need = lib.stattn_verify_draft_workspace(b, j, v)
-    work = _empty((need,), dtype=_U8, device=device) if need else None        # alive until the launches are enqueued
+    work = draft.new_empty((need,), dtype=_U8) if need else None        # alive until the launches are enqueued
     rc = lib.stattn_verify_draft(dev, _raw_stream(dev), draft.data_ptr(), db, target.data_ptr(), tb, tj, pp, pb, pj, dtype, accept_u.data_ptr(), ub,
                                  draw_u.data_ptr(), pl, b, j, v, words.data_ptr(), j + 1, accepted.data_ptr(), work.data_ptr() if need else None, need)
     if rc:
