@@ -59,7 +59,7 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
     CHK(getbuf_t(h, "dr_lg", (size_t)P * M * Vp, &lg)); CHK(getbuf_t(h, "dr_p", (size_t)P * M * Vp, &p));
     CHK(getbuf_t(h, "dr_head", (size_t)V * (mx4_kp(E) / 2), &hc)); CHK(getbuf_t(h, "dr_head_scales", (size_t)V * (mx4_kp(E) / 32), &hsc));
     double* vsums;
-    CHK(getbuf_t(h, "dr_sums", (size_t)M * verify_split(M, V) * 16, &vsums));
+    CHK(getbuf_t(h, "dr_sums", (size_t)M * 256, &vsums));
     DraftState d{};
     d.M = M; d.D = D; d.k = draft; d.maxlen = maxlen; d.x = xs;
     CHK(getbuf_t(h, "dr_h", (size_t)M * D, &d.h)); CHK(getbuf_t(h, "dr_c", (size_t)M * D, &d.c)); CHK(getbuf_t(h, "dr_info", (size_t)M, &d.info));

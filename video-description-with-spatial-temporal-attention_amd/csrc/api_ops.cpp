@@ -147,7 +147,7 @@ int stattn_mx4_linear(int device, void* stream, const void* x, int dtype, int64_
 size_t stattn_verify_draft_workspace(int64_t b, int64_t j, int64_t v) {
     (void)j;
     const int n = b > 0 ? verify_split(b, v) : 1;
-    return n > 1 ? (size_t)b * n * 16 * sizeof(double) : 0;
+    return n > 1 ? (size_t)b * 256 * sizeof(double) : 0;
 }
 
 int stattn_verify_draft(int device, void* stream, const int64_t* draft, int64_t draft_ld, const void* target, int64_t target_b,

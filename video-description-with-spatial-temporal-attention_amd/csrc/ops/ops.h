@@ -48,15 +48,15 @@ struct VerifyArgs {
     const int32_t* lens;                                     // or null: every draft has j words
     int64_t b; int j; int64_t v;
     int64_t* words; int64_t words_ld; int32_t* accepted;
-    int split; double* sums;                                 // workgroups that sum a caption's rows, and [b][split * 16] sums; 1: none
+    int split; double* sums;                                 // workgroups that sum a caption's rows, and [b][256] sums; 1: none
 };
-constexpr int VERIFY_SPLIT = 16;
-// Long rows of few captions: several workgroups a caption, up to two a CU in all.  (One takes 20 us for 128000 words; a launch more takes
-// the GPU 3 us and a caller 3.5, so rows under 32768 words stay with one.)
+// Long rows of few captions: several workgroups a caption, one a CU in all.  (1 x 128000 words: 12 us instead of 18, 64 x 128000 in bf16 14
+// instead of 21; 1 x 64000 11.9 and 12.5, of which a caller has 13.8 and 12.2, a launch more taking 3.5 us of its time; 128 x 128000: 29
+// and 27.)
 inline int verify_split(int64_t b, int64_t v) {
-    if (v < 32768 || b > 256) return 1;
+    if (v < 98304 || b > 64) return 1;
     int n = 1;
-    while (n < VERIFY_SPLIT && b * n < 256 && v / (n * 32) >= 1024) n *= 2;
+    while (n < 16 && b * n < 256) n *= 2;
     return n;
 }
 hipError_t launch_verify_draft(hipStream_t s, const VerifyArgs& a);

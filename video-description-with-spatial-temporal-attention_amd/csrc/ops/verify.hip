@@ -12,10 +12,22 @@ namespace stattn {
 template <OpType T>
 __device__ __forceinline__ double prob(const void* base, int64_t i) { return (double)(float)static_cast<const typename Elem<T>::type*>(base)[i]; }
 
+// Sum over the wave on the vector pipe: lanes meet by DPP moves (quad swaps, half-row and row mirrors, then the rows' totals are handed on);
+// by LDS permutes, twelve dependent ones for a 64-bit value, it took longer than summing 512 words.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp64(double old, double v) {
+    const int2 o = __builtin_bit_cast(int2, old), x = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_update_dpp(o.x, x.x, CTRL, ROWS, 0xF, false), __builtin_amdgcn_update_dpp(o.y, x.y, CTRL, ROWS, 0xF, false)));
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    v += dpp64<0xB1, 0xF>(v, v);            // quad_perm [1, 0, 3, 2]
+    v += dpp64<0x4E, 0xF>(v, v);            // quad_perm [2, 3, 0, 1]
+    v += dpp64<0x141, 0xF>(v, v);           // row_half_mirror: every lane the sum of its eight
+    v += dpp64<0x140, 0xF>(v, v);           // row_mirror: of its row of sixteen
+    v += dpp64<0x142, 0xA>(0.0, v);         // row_bcast 15: rows 1 and 3 add the row before
+    v += dpp64<0x143, 0xC>(0.0, v);         // row_bcast 31: row 3 adds the first half; lane 63 has all
+    const int2 x = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(x.x, 63), __builtin_amdgcn_readlane(x.y, 63)));
 }
 
 // One caption's weights over a stretch of the vocabulary: p alone, p without the one word that a certain proposal has all its mass on, or
@@ -36,8 +48,7 @@ struct Weights {
     __device__ __forceinline__ double at(int64_t i) const { return q ? over((float)p[i], (float)q[i]) : i == certain ? over((float)p[i], 1.f) : over((float)p[i]); }
 
     // Sum of the weights from `from` to `to`, this lane's share of the wave's walk; K requests on their way.  The lanes take eight
-    // neighbours each.  The conversions to 64 bits are what it costs: over a
-    // proposal some 90 cycles for 64 words, so a CU takes 128000 words in 20 us.
+    // neighbours each.
     template <bool Q>
     __device__ __forceinline__ double walk(int64_t from, int64_t to, int lane) const {
         constexpr int K = sizeof(E) == 4 ? 2 : 4;       // (sixteen waves leave 128 registers each)
@@ -62,6 +73,40 @@ struct Weights {
         }
         return sum;
     }
+    // The sums of stretches k, k + stride, ... of `n` stretches of 512 words into all[]; K of them on their way.
+    template <bool Q>
+    __device__ __forceinline__ void chunks(int k0, int stride, int n, int64_t v, int lane, double* all) const {
+        constexpr int K = 2;
+        for (; k0 < n; k0 += K * stride) {
+            Eight<T> a[K], b[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int64_t c = (int64_t)(k0 + k * stride) * 512 + 8 * lane;
+                const int here = (int)min(v - c, (int64_t)8);
+                a[k].take(p + c, here);
+                if (Q) b[k].take(q + c, here);
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int at_ = k0 + k * stride;
+                if (at_ >= n) break;
+                float x[8], y[8];
+                a[k].put(x);
+                if (Q) b[k].put(y);
+                double s = 0.0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s += Q ? over(x[j], y[j]) : over(x[j]);
+                if (!Q && certain >= (int64_t)at_ * 512 && certain < (int64_t)at_ * 512 + 512) {     // (the same for the wave, and rare)
+                    const int64_t c = (int64_t)at_ * 512 + 8 * lane;
+                    s = 0.0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) s += c + j == certain ? over(x[j], 1.f) : over(x[j]);
+                }
+                s = wave_sum64(s);
+                if (lane == 0) all[at_] = s;
+            }
+        }
+    }
     __device__ __forceinline__ double sum(int64_t from, int64_t to, int lane) const {
         if (q) return wave_sum64(walk<true>(from, to, lane));
         if (certain < from || certain >= to) return wave_sum64(walk<false>(from, to, lane));
@@ -74,13 +119,15 @@ struct Weights {
     }
 };
 
-// The first word of caption i's draft that is refused, or its length; every wave finds it for itself, a lane a word.
+// The first word of caption i's draft that is refused, or its length; every wave finds it for itself, a lane a word.  Words are read
+// whether they count or not, so that the length need not be there first.
 template <OpType T>
-__device__ __forceinline__ int first_refused(const VerifyArgs& a, int64_t i, int len, int lane) {
-    for (int j0 = 0; j0 < len; j0 += 64) {
+__device__ __forceinline__ int first_refused(const VerifyArgs& a, int64_t i, int& len, int lane) {
+    len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j;
+    for (int j0 = 0; j0 < a.j; j0 += 64) {
         const int j = j0 + lane;
         bool kept = true;
-        if (j < len) {
+        if (j < a.j) {
             const int64_t d = a.draft[i * a.draft_b + j * a.draft_j];
             kept = d >= 0 && d < a.v;
             if (kept) {
@@ -90,7 +137,8 @@ __device__ __forceinline__ int first_refused(const VerifyArgs& a, int64_t i, int
             }
         }
         const unsigned long long refused = __ballot(!kept);
-        if (refused) return __builtin_amdgcn_readfirstlane(j0 + __builtin_ctzll(refused));
+        if (refused) return min(__builtin_amdgcn_readfirstlane(j0 + __builtin_ctzll(refused)), len);
+        if (j0 + 64 >= len) break;
     }
     return len;
 }
@@ -103,8 +151,24 @@ __device__ __forceinline__ Weights<T> weights_at(const VerifyArgs& a, int64_t i,
     w.certain = n < len && !a.proposal ? a.draft[i * a.draft_b + n * a.draft_j] : -1;
     return w;
 }
-// The vocabulary in `n` stretches: multiples of 512 words, as many as 64 lanes take at a time.
+// The length of at most `n` stretches of the vocabulary: multiples of 512 words, as many as 64 lanes take at a time.
 __device__ __forceinline__ int64_t stretch(int64_t v, int n) { return ((v + n - 1) / n + 511) & ~(int64_t)511; }
+constexpr int STRETCHES = 256, NW16 = 16;
+// This wave's share (every `stride`-th) of the sums of all stretches.
+template <OpType T>
+__device__ __forceinline__ void sum_stretches(const Weights<T>& w, int64_t v, int k0, int stride, int lane, double* all) {
+    const int64_t step = stretch(v, STRETCHES);
+    const int n = (int)((v + step - 1) / step);
+    if (step == 512) {
+        if (w.q) w.template chunks<true>(k0, stride, n, v, lane, all);
+        else w.template chunks<false>(k0, stride, n, v, lane, all);
+        return;
+    }
+    for (int k = k0; k < n; k += stride) {
+        const double s = w.sum(k * step, min((k + 1) * step, v), lane);
+        if (lane == 0) all[k] = s;
+    }
+}
 // Running sums of the stretches, four neighbours a lane (a loop over them, one dependent read and addition after the other, took longer
 // than reading the rows).
 struct Running {
@@ -139,64 +203,56 @@ struct Running {
     }
 };
 
-constexpr int NW16 = 16;
-
 // The stretches' sums of long rows by several workgroups a caption (blockIdx.x of gridDim.x), for verify_kernel to go on from.
 template <OpType T>
 __global__ __launch_bounds__(64 * NW16) void verify_sums_kernel(VerifyArgs a) {
     const int64_t i = blockIdx.y;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ns = gridDim.x * NW16, k = blockIdx.x * NW16 + wave;
-    const int len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j, n = first_refused<T>(a, i, len, lane);
-    const Weights<T> w = weights_at<T>(a, i, n, len);
-    const int64_t step = stretch(a.v, ns), lo = min(k * step, a.v), hi = min(lo + step, a.v);
-    const double mine = lo < hi ? w.sum(lo, hi, lane) : 0.0;
-    if (lane == 0) a.sums[i * ns + k] = mine;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int len;
+    const int n = first_refused<T>(a, i, len, lane);
+    sum_stretches<T>(weights_at<T>(a, i, n, len), a.v, blockIdx.x * NW16 + wave, gridDim.x * NW16, lane, a.sums + i * STRETCHES);
 }
 
-// One workgroup of NW waves a caption.  The vocabulary is cut into NW stretches, a wave sums one (or the sums of `split` * 16 stretches are
-// there already); the stretch that the draw falls into is cut again if it is long, and one wave walks the rest word by word.  That reads
-// the rows once and a sixteenth (a 256th) of them again, and no sum's order depends on anything but v and b, so results repeat.  Bound: at
-// one caption the chain of dependent reads (draft -> probabilities -> rows -> stretch), at many reading two rows each.
+// One workgroup of NW waves a caption.  The vocabulary is cut into stretches of 512 words (longer ones from 131072 words on: 256 at most),
+// whose sums the waves share out (or verify_sums_kernel has left); in the stretch that the draw falls into one wave goes word by word.
+// That reads the rows once and one stretch again, and no sum's order depends on anything but v, so results repeat.  Bound: at one
+// caption the chain of dependent reads (draft -> probabilities -> rows -> stretch), at many reading two rows each.
 template <OpType T, int NW>
 __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
-    __shared__ double given[VERIFY_SPLIT * NW16];
-    __shared__ double part[2][2][NW];       // [turn][level]: never written again while a wave may still read it
+    __shared__ double all[2][STRETCHES];    // [turn]: never written again while a wave may still read it
+    __shared__ double part[2][NW];
     const int64_t i = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int len = a.lens ? min(max(a.lens[i], 0), a.j) : a.j, n = first_refused<T>(a, i, len, lane);
-    Weights<T> w = weights_at<T>(a, i, n, len);
     const double u = (double)a.draw_u[i];
+    int len;
+    const int n = first_refused<T>(a, i, len, lane);
+    Weights<T> w = weights_at<T>(a, i, n, len);
 
     int64_t word = -1;
     for (int turn = 0; turn < 2; ++turn) {
-        const bool there = turn == 0 && a.split > 1;
-        const int ns = there ? a.split * NW16 : NW;
-        int64_t from = 0, to = a.v, step = stretch(a.v, ns);
-        double base = 0.0, t = 0.0;
-        bool any = false;
-        for (int level = 0; level < 2; ++level) {
-            if (level == 0 && there) {
-                for (int k = tid; k < ns; k += 64 * NW) given[k] = a.sums[i * ns + k];
-            } else {
+        int64_t step = stretch(a.v, STRETCHES);
+        const int ns = (int)((a.v + step - 1) / step);
+        if (turn == 0 && a.split > 1) {
+            if (tid < ns) all[0][tid] = a.sums[i * STRETCHES + tid];
+        } else {
+            sum_stretches<T>(w, a.v, wave, NW, lane, all[turn]);
+        }
+        __syncthreads();
+        const Running run(all[turn], ns, lane);
+        const double total = run.total(), t = u * total;
+        double base = 0.0;
+        const bool any = total > 0.0;
+        if (any) {
+            int64_t from = min(run.passes(t, base, lane) * step, a.v), to = min(from + step, a.v);
+            if (step > 2048) {               // a long stretch is cut once more
+                step = stretch(to - from, NW);
                 const int64_t lo = min(from + wave * step, to), hi = min(lo + step, to);
                 const double mine = lo < hi ? w.sum(lo, hi, lane) : 0.0;
-                if (lane == 0) part[turn][level][wave] = mine;
+                if (lane == 0) part[turn][wave] = mine;
+                __syncthreads();
+                from = min(from + max(Running(part[turn], NW, lane).passes(t, base, lane), 0) * step, to);
+                to = min(from + step, to);
             }
-            __syncthreads();
-            const double* all = level == 0 && there ? given : part[turn][level];
-            const Running run(all, level == 0 ? ns : NW, lane);
-            if (level == 0) {
-                const double total = run.total();
-                any = total > 0.0;
-                if (!any) break;
-                t = u * total;
-            }
-            from = min(from + max(run.passes(t, base, lane), 0) * step, to);
-            to = min(from + step, to);
-            if (step <= 2048) break;
-            step = stretch(to - from, NW);
-        }
-        if (any) {
             if (wave == 0) {                 // word by word: eight neighbours a lane, 512 at a time
                 for (int64_t c0 = from; c0 < to; c0 += 512) {
                     const int64_t c = c0 + 8 * lane;
