@@ -107,7 +107,7 @@ int stattn_mx4_matmul(int device, void* stream, const void* a_codes, const void*
 }
 
 // Few rows: one launch in which every workgroup rounds x for itself, instead of two with x's 4-bit form between them.  Up to 32768
-// values of x that takes the GPU little longer (1 x 12000 x 512: 3.8 us against 5.1; 32: 6.0 against 5.6; 64: 8.9 against 5.8; beyond,
+// values of x that takes the GPU little longer (1 x 12000 x 512: 3.5 us against 5.1; 32: 6.0 against 5.6; 64: 9.1 against 5.8; beyond,
 // 64 x 20000 x 1024: 18.5 against 7.4) and saves the caller a launch and a workspace, 4.5 us of its time.  Rows whose last eight are
 // partial load one by one in between (64 x 12000 x 511: 12): up to 16384.
 static bool few_rows(int64_t m, int64_t k) { return m <= 64 && m * k <= (k % 8 ? 16384 : 32768); }

@@ -1,6 +1,6 @@
 // y = x w^T + bias for few rows of x: x is brought into 4 bits inside the launch, w (n, k) in 4 bits is read once.
 // What bounds it is reading w, 17/32 byte an element, and below some megabytes the latency of doing so: 1 x 12000 x 512 (3.3 MB) takes
-// 3.8 us, 5 x 20000 x 1024 (11 MB) 7.2, 64 x 12000 x 512 8.9 -- there every workgroup's rounding of x counts.  With 32 or 64 rows of w a
+// 3.5 us, 5 x 20000 x 1024 (11 MB) 6.5, 64 x 12000 x 512 9.1 -- there every workgroup's rounding of x counts.  With 32 or 64 rows of w a
 // wave instead of 16, so that fewer workgroups round x, 160 x 12000 x 512 took 12.0 and 17.3 us instead of 14.6; two launches (the
 // form of x written once, then mx4_gemm.hip) take 7.6 and are used from there on.
 #include "mx4_inl.h"
@@ -12,8 +12,10 @@ namespace stattn {
 // v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds row l % 16 and block l / 16 of four of an operand.  The workgroup's 16 MT rows of x are
 // rounded into LDS once, KC columns at a time, in that layout (row after row, 16 bytes further each, so that the sixteen lanes of a
 // read meet sixteen slots of four banks).  A wave owns 16 rows of w and streams them from memory into registers, as they are, U steps
-// of 128 columns ahead, the first of them before x is rounded.  KS = 4: the four waves share 16 rows of w, every fourth step each, and
-// add up through LDS: for heads with few rows, where a wave a group would leave most of the chip without one.
+// of 128 columns ahead, the first of them asked for behind the first values of x and on their way while those are rounded (asked for in
+// front of them, they had to arrive first, since loads come back in order: 5 x 20000 x 1024 took 7.1 us instead of 6.5).  KS = 4: the
+// four waves share 16 rows of w, every fourth step each, and add up through LDS: for heads with few rows, where a wave a group would
+// leave most of the chip without one.
 constexpr int U = 8;
 
 template <OpType T, int MT, int KS>
@@ -51,12 +53,11 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(Mx4LinearArgs p) {
     const int first = KS == 1 ? 0 : wave;
     for (int c0 = 0; c0 < steps; c0 += KC / 128) {                  // KC columns of x
         const int cs = min(steps - c0, KC / 128);
-        fetch(c0 + first);
         if (c0) __syncthreads();
         const int words = cs * 16, total = rows * words;            // eight columns each; all counts are multiples of 4, so a quad is whole
         auto round_x = [&](auto requests) {                         // that many requests of a lane on their way
             constexpr int Q = decltype(requests)::value;
-            for (int i0 = tid; i0 - tid < total; i0 += 256 * Q) {
+            auto some = [&](int i0, auto meanwhile) {
                 Eight<T> x[Q];
                 int at[Q], row[Q];
 #pragma unroll
@@ -67,6 +68,9 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(Mx4LinearArgs p) {
                     const int64_t c = (int64_t)c0 * 128 + at[q] * 8;
                     x[q].take(static_cast<const E*>(p.x) + (m0 + row[q]) * p.ldx + c, (int)(p.w.cols - c));
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                meanwhile();
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int q = 0; q < Q; ++q) {
                     float v[8];
@@ -75,7 +79,9 @@ __global__ __launch_bounds__(256) void mx4_linear_kernel(Mx4LinearArgs p) {
                     *reinterpret_cast<unsigned*>(xc + row[q] * RS + at[q] * 4) = mx4_codes8(v, byte);
                     if ((at[q] & 3) == 0) xs[row[q] * SS + (at[q] >> 2)] = (uint8_t)byte;
                 }
-            }
+            };
+            some(tid, [&]() { fetch(c0 + first); });
+            for (int i0 = tid + 256 * Q; i0 - tid < total; i0 += 256 * Q) some(i0, []() {});
         };
         if (total <= 256) round_x(std::integral_constant<int, 1>());
         else if (MT == 1 && total <= 1024) round_x(std::integral_constant<int, 4>());
