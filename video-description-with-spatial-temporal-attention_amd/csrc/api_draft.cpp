@@ -8,10 +8,10 @@
 #include "steps.h"
 #include "ops/ops.h"
 
-extern "C" {
+#include <new>
 
-int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl, const float* ctxm, int T,
-                          int K, int draft, int maxlen, const float* uniforms, int64_t* out_tokens, float* out_scores, int32_t* out_lens,
+static int sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl, const float* ctxm, int T, int K,
+                          int draft, int maxlen, const float* uniforms, int64_t* out_tokens, float* out_scores, int32_t* out_lens,
                           int32_t* out_drafted, int32_t* out_kept) {
     const bool resident = !ctxg && !ctxg_mask && !ctxl && !ctxm;
     if (!h || nvid < 1 || nvid > 16 || (!resident && (!ctxg || !ctxg_mask || !ctxl || !ctxm)) || T <= 0 || K <= 0 || draft < 1 || draft > 8 ||
@@ -228,4 +228,12 @@ int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
     return STATTN_OK;
 }
 
-}  // extern "C"
+extern "C" int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl, const float* ctxm,
+                                     int T, int K, int draft, int maxlen, const float* uniforms, int64_t* out_tokens, float* out_scores,
+                                     int32_t* out_lens, int32_t* out_drafted, int32_t* out_kept) {
+    try {
+        return sample_drafted(h, nvid, ctxg, ctxg_mask, ctxl, ctxm, T, K, draft, maxlen, uniforms, out_tokens, out_scores, out_lens, out_drafted, out_kept);
+    } catch (const std::bad_alloc&) {       // (the numbers of a call, 4 maxlen (2 draft + 1) nvid bytes, when the handle draws them)
+        return fail(h, STATTN_EHIP, "sample_drafted: out of host memory");
+    }
+}
