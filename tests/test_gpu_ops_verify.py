@@ -40,7 +40,7 @@ def check(ops, args, lens=None):
 
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("b,j,v", [(1, 0, 1), (1, 1, 1), (1, 1, 2), (3, 2, 7), (1, 4, 63), (5, 5, 64), (2, 3, 1000), (64, 5, 1025), (1, 4, 12000), (7, 8, 4099),
-                                   (33, 1, 20000), (3, 70, 500), (2, 2, 50257), (1, 3, 128000), (300, 2, 37), (4, 3, 200001)])
+                                   (33, 1, 20000), (3, 70, 500), (2, 2, 50257), (1, 3, 128000), (300, 2, 37), (4, 3, 200001), (70, 1, 98304)])
 def test_words_and_counts(ops, dt, b, j, v):
     args = make(b, j, v, DTYPES[dt], b + 3 * j + 7 * v)
     check(ops, args)
@@ -124,7 +124,7 @@ def test_no_captions(ops):
     assert words.shape == (0, 4) and acc.shape == (0,)
 
 
-@pytest.mark.parametrize("b,j,v", [(1, 4, 300), (4, 3, 60000)])
+@pytest.mark.parametrize("b,j,v", [(1, 4, 300), (4, 3, 60000), (2, 2, 98305)])
 def test_captured_and_replayed_and_on_other_streams(ops, b, j, v):
     args = make(b, j, v, torch.float32, 8)
     ops.verify_draft(*args)

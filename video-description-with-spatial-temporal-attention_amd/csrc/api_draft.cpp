@@ -169,7 +169,7 @@ static int sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
         }
         HIPCHK(h, launch_softmax_draw(s, DrawArgs{lg, p, Vp, V, P * M, nullptr, nullptr, nullptr, nullptr, 0}));
         VerifyArgs v{};
-        v.split = verify_split(M, V); v.sums = vsums;
+        v.split = verify_split(M, V, OP_F32); v.sums = vsums;
         v.draft = xs + M; v.draft_b = 1; v.draft_j = M;
         v.target = p; v.target_b = Vp; v.target_j = (int64_t)M * Vp; v.proposal = q; v.proposal_b = Vp; v.proposal_j = (int64_t)M * Vp;
         v.type = OP_F32; v.accept_u = d.u + (size_t)draft * M; v.accept_b = 1; v.accept_j = M; v.draw_u = d.u + (size_t)2 * draft * M;

@@ -146,7 +146,7 @@ int stattn_mx4_linear(int device, void* stream, const void* x, int dtype, int64_
 
 size_t stattn_verify_draft_workspace(int64_t b, int64_t j, int64_t v) {
     (void)j;
-    const int n = b > 0 ? verify_split(b, v) : 1;
+    const int n = b > 0 ? verify_split(b, v, OP_BF16) : 1;      // (32 bits are split for fewer captions)
     return n > 1 ? (size_t)b * 256 * sizeof(double) : 0;
 }
 
@@ -168,7 +168,7 @@ int stattn_verify_draft(int device, void* stream, const int64_t* draft, int64_t 
     const OnDevice on(device);
     if (on.err != hipSuccess) return launched("verify_draft", on.err);
     const VerifyArgs a{draft, draft_ld, 1, target, target_b, target_j, proposal, proposal_b, proposal_j, (OpType)dtype, accept_u, accept_ld, 1,
-                       draw_u, lens, b, (int)j, v, words, words_ld, accepted, verify_split(b, v), static_cast<double*>(workspace)};
+                       draw_u, lens, b, (int)j, v, words, words_ld, accepted, verify_split(b, v, (OpType)dtype), static_cast<double*>(workspace)};
     return launched("verify_draft", launch_verify_draft(static_cast<hipStream_t>(stream), a));
 }
 

@@ -51,10 +51,11 @@ struct VerifyArgs {
     int split; double* sums;                                 // workgroups that sum a caption's rows, and [b][256] sums; 1: none
 };
 // Long rows of few captions: several workgroups a caption, one a CU in all.  (1 x 128000 words: 12 us instead of 18, 64 x 128000 in bf16 14
-// instead of 21; 1 x 64000 11.9 and 12.5, of which a caller has 13.8 and 12.2, a launch more taking 3.5 us of its time; 128 x 128000: 29
-// and 27.)
-inline int verify_split(int64_t b, int64_t v) {
-    if (v < 98304 || b > 64) return 1;
+// instead of 21; 1 x 64000 11.9 and 12.5, of which a caller has 13.8 and 12.2, a launch more taking 3.5 us of its time.)  With 128
+// captions in 16 bits half the CUs are bound by arithmetic and two workgroups help (128 x 128000: 18 us instead of 21); in 32 bits they
+// wait for memory either way (24.4 and 23.5).
+inline int verify_split(int64_t b, int64_t v, OpType type) {
+    if (v < 98304 || b > (type == OP_F32 ? 64 : 128)) return 1;
     int n = 1;
     while (n < 16 && b * n < 256) n *= 2;
     return n;

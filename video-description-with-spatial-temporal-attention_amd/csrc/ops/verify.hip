@@ -5,7 +5,7 @@
 // which makes the kept words and the drawn one a sample of the target's distribution whatever the proposal is.
 // Products and sums are in 64 bits: u q is then exact for 32-bit inputs, and a word next to a border of the running sum does not
 // depend on the order of 32-bit roundings.
-// 1 caption x 12000 words 7 us, 64 x 20000 in fp32 8.8, 128 x 128000 in bf16 21 (66 MB, 3.1 TB/s: the conversions to 64 bits on half the CUs).
+// 1 caption x 12000 words 7 us, 64 x 20000 in fp32 8.8, 128 x 128000 in bf16 18 (66 MB, 3.7 TB/s), 128 x 250000 28 (4.6 TB/s).
 #include "mx4_inl.h"
 
 namespace stattn {
@@ -52,7 +52,7 @@ struct Weights {
     // neighbours each.
     template <bool Q>
     __device__ __forceinline__ double walk(int64_t from, int64_t to, int lane) const {
-        constexpr int K = sizeof(E) == 4 ? 2 : 4;       // (sixteen waves leave 128 registers each)
+        constexpr int K = 2;            // (stretches of 1024 words are the most frequent here; with 4, 128 x 250000 in bf16 took 41 us instead of 28)
         double sum = 0.0;
         for (int64_t c0 = from; c0 < to; c0 += 512 * K) {
             Eight<T> a[K], b[K];
