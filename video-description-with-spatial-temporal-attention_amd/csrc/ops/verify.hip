@@ -5,7 +5,7 @@
 // which makes the kept words and the drawn one a sample of the target's distribution whatever the proposal is.
 // Products and sums are in 64 bits: u q is then exact for 32-bit inputs, and a word next to a border of the running sum does not
 // depend on the order of 32-bit roundings.
-// 1 caption x 12000 words 7 us, 64 x 20000 in fp32 8.8, 128 x 128000 in bf16 18 (66 MB, 3.7 TB/s), 128 x 250000 28 (4.6 TB/s).
+// 1 caption x 12000 words 7 us, 64 x 20000 in fp32 8.8, 128 x 128000 in bf16 19 (66 MB, 3.5 TB/s), 128 x 250000 28 (4.6 TB/s).
 #include "mx4_inl.h"
 
 namespace stattn {
