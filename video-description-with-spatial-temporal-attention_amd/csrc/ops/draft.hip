@@ -1,13 +1,14 @@
 // Kernels of drafted sampling (api_draft.cpp): distributions and draws of the drafts, and per caption the state behind the kept words, the
 // words, the next round's numbers.
 #include "mx4_inl.h"
+#include "wave_inl.h"
 
 namespace stattn {
 
 // One workgroup of 16 waves a row, a stretch of the row (a multiple of 512 words) for each wave, eight neighbours a lane.  Three walks of
 // it, the second and third from the caches: the largest logit, the sum, the probabilities -- whose own sums over the stretches (in 64 bits)
 // then say where a draw falls, and the first wave looks there word by word.  A row of 20000 words is 20 values a lane: what counts is the
-// chain of reads (9.6 us; the 256-lane softmax of the other paths takes 41 us for such a row, and the draw was another launch).
+// chain of reads (8.6 us; the 256-lane softmax of the other paths takes 41 us for such a row, and the draw was another launch).
 __global__ __launch_bounds__(1024) void softmax_draw_kernel(DrawArgs a) {
     constexpr int NW = 16;
     __shared__ float top[NW], sums[NW];
@@ -31,8 +32,7 @@ __global__ __launch_bounds__(1024) void softmax_draw_kernel(DrawArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);
     });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    m = wave_max(m);
     if (lane == 0) top[wave] = m;
     __syncthreads();
     for (int k = 0; k < NW; ++k) m = fmaxf(m, top[k]);
@@ -41,8 +41,7 @@ __global__ __launch_bounds__(1024) void softmax_draw_kernel(DrawArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += __expf(v[j] - m);
     });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    sum = wave_sum(sum);
     if (lane == 0) sums[wave] = sum;
     __syncthreads();
     sum = 0.f;
@@ -57,20 +56,17 @@ __global__ __launch_bounds__(1024) void softmax_draw_kernel(DrawArgs a) {
         reinterpret_cast<float4*>(p + c)[1] = make_float4(e[4], e[5], e[6], e[7]);
     });
     if (!a.u) return;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
+    mine = wave_sum(mine);
     if (lane == 0) part[wave] = mine;
     __syncthreads();
     if (wave) return;
     // the stretch that the draw falls into: a lane a stretch
     const double own = lane < NW ? part[lane] : 0.0;
-    double upto = own;
-#pragma unroll
-    for (int o = 1; o < NW; o <<= 1) { const double y = __shfl_up(upto, o, 64); if (lane >= o) upto += y; }
-    const double t = (double)a.u[blockIdx.x] * __shfl(upto, NW - 1, 64);
+    const double upto = wave_scan(own);
+    const double t = (double)a.u[blockIdx.x] * from_lane(upto, NW - 1);
     const unsigned long long over16 = __ballot(lane < NW && own > 0.0 && upto > t), with16 = __ballot(own > 0.0);
     const int last = over16 ? __builtin_ctzll(over16) : with16 ? 63 - __builtin_clzll(with16) : 0;
-    double base = __shfl(upto - own, last, 64);
+    double base = from_lane(upto - own, last);
     const int from = min(last * step, a.v), to = min(from + step, a.v);
     int word = 0;                                       // (a row of NaNs draws word 0)
     for (int c0 = from; c0 < to; c0 += 512) {
@@ -79,9 +75,7 @@ __global__ __launch_bounds__(1024) void softmax_draw_kernel(DrawArgs a) {
         double eight = 0.0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) { e[j] = i + j < to ? p[i + j] : 0.f; eight += (double)e[j]; }
-        double incl = eight;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const double y = __shfl_up(incl, o, 64); if (lane >= o) incl += y; }
+        const double incl = wave_scan(eight);
         double run = base + (incl - eight);
         int first = -1, some = -1;
 #pragma unroll
@@ -90,9 +84,9 @@ __global__ __launch_bounds__(1024) void softmax_draw_kernel(DrawArgs a) {
             if (e[j] > 0.f) { some = i + j; if (run > t && first < 0) first = i + j; }
         }
         const unsigned long long over = __ballot(first >= 0), with = __ballot(some >= 0);
-        if (over) { word = __shfl(first, __builtin_ctzll(over), 64); break; }
-        if (with) word = __shfl(some, 63 - __builtin_clzll(with), 64);
-        base += __shfl(incl, 63, 64);
+        if (over) { word = from_lane(first, __builtin_ctzll(over)); break; }
+        if (with) word = from_lane(some, 63 - __builtin_clzll(with));
+        base += from_lane(incl, 63);
     }
     if (lane == 0) a.words[blockIdx.x] = word;
     for (int i = lane; i < a.dim / 4; i += 64)
@@ -147,8 +141,8 @@ __global__ __launch_bounds__(1024) void draft_commit_kernel(DraftState d, const 
     if (bad && __builtin_ctzll(bad) < take) take = __builtin_ctzll(bad);
     if (t < take) d.tokens[(int64_t)m * d.maxlen + f.len + t] = w;
     float score = f.score;
-    for (int j = 0; j < take; ++j) score += __shfl(pw, j, 64);
-    const int64_t last = __shfl(w, n, 64);
+    for (int j = 0; j < take; ++j) score += from_lane(pw, j);
+    const int64_t last = from_lane(w, n);
     if (t == 0) {
         f.drafted += d.k; f.kept += n; ++f.rounds;
         f.len += take; f.score = score;

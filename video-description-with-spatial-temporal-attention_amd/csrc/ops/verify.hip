@@ -5,31 +5,14 @@
 // which makes the kept words and the drawn one a sample of the target's distribution whatever the proposal is.
 // Products and sums are in 64 bits: u q is then exact for 32-bit inputs, and a word next to a border of the running sum does not
 // depend on the order of 32-bit roundings.
-// 1 caption x 12000 words 7 us, 64 x 20000 in fp32 8.8, 128 x 128000 in bf16 19 (66 MB, 3.5 TB/s), 128 x 250000 28 (4.6 TB/s).
+// 1 caption x 12000 words 7 us, 64 x 20000 in fp32 7.9, 128 x 128000 in bf16 18 (66 MB, 3.7 TB/s), 128 x 250000 28 (4.6 TB/s).
 #include "mx4_inl.h"
+#include "wave_inl.h"
 
 namespace stattn {
 
 template <OpType T>
 __device__ __forceinline__ double prob(const void* base, int64_t i) { return (double)(float)static_cast<const typename Elem<T>::type*>(base)[i]; }
-
-// Sum over the wave on the vector pipe: lanes meet by DPP moves (quad swaps, half-row and row mirrors, then the rows' totals are handed on);
-// by LDS permutes, twelve dependent ones for a 64-bit value, it took longer than summing 512 words.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp64(double old, double v) {
-    const int2 o = __builtin_bit_cast(int2, old), x = __builtin_bit_cast(int2, v);
-    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_update_dpp(o.x, x.x, CTRL, ROWS, 0xF, false), __builtin_amdgcn_update_dpp(o.y, x.y, CTRL, ROWS, 0xF, false)));
-}
-__device__ __forceinline__ double wave_sum64(double v) {
-    v += dpp64<0xB1, 0xF>(v, v);            // quad_perm [1, 0, 3, 2]
-    v += dpp64<0x4E, 0xF>(v, v);            // quad_perm [2, 3, 0, 1]
-    v += dpp64<0x141, 0xF>(v, v);           // row_half_mirror: every lane the sum of its eight
-    v += dpp64<0x140, 0xF>(v, v);           // row_mirror: of its row of sixteen
-    v += dpp64<0x142, 0xA>(0.0, v);         // row_bcast 15: rows 1 and 3 add the row before
-    v += dpp64<0x143, 0xC>(0.0, v);         // row_bcast 31: row 3 adds the first half; lane 63 has all
-    const int2 x = __builtin_bit_cast(int2, v);
-    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(x.x, 63), __builtin_amdgcn_readlane(x.y, 63)));
-}
 
 // One caption's weights over a stretch of the vocabulary: p alone, p without the one word that a certain proposal has all its mass on, or
 // p over q.
@@ -103,20 +86,20 @@ struct Weights {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) s += c + j == certain ? over(x[j], 1.f) : over(x[j]);
                 }
-                s = wave_sum64(s);
+                s = wave_sum(s);
                 if (lane == 0) all[at_] = s;
             }
         }
     }
     __device__ __forceinline__ double sum(int64_t from, int64_t to, int lane) const {
-        if (q) return wave_sum64(walk<true>(from, to, lane));
-        if (certain < from || certain >= to) return wave_sum64(walk<false>(from, to, lane));
+        if (q) return wave_sum(walk<true>(from, to, lane));
+        if (certain < from || certain >= to) return wave_sum(walk<false>(from, to, lane));
         // A certain proposal's word weighs p - 1 (0 unless p is over 1), not p.  Taken back from the sum it would leave a rounding behind,
         // so the 512 words around it are summed without it.
         const int64_t c0 = from + ((certain - from) & ~(int64_t)511), c1 = min(c0 + 512, to);
         double s = walk<false>(from, c0, lane) + walk<false>(c1, to, lane);
         for (int64_t c = c0 + lane; c < c1; c += 64) s += at(c);
-        return wave_sum64(s);
+        return wave_sum(s);
     }
 };
 
@@ -178,11 +161,9 @@ struct Running {
         double own = 0.0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { x[j] = 4 * lane + j < n ? all[4 * lane + j] : 0.0; own += x[j]; }
-        incl = own;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const double y = __shfl_up(incl, o, 64); if (lane >= o) incl += y; }
+        incl = wave_scan(own);
     }
-    __device__ __forceinline__ double total() const { return __shfl(incl, 63, 64); }
+    __device__ __forceinline__ double total() const { return from_lane(incl, 63); }
     // The stretch in which the running sum from `base` on passes t, and (in `base`) the sum in front of it; where roundings leave none,
     // the last with any weight.
     __device__ __forceinline__ int passes(double t, double& base, int lane) const {
@@ -199,8 +180,8 @@ struct Running {
         }
         const unsigned long long over = __ballot(first >= 0), with = __ballot(some >= 0);
         const int from = over ? __builtin_ctzll(over) : with ? 63 - __builtin_clzll(with) : 0;
-        base = __shfl(over ? at_first : at_some, from, 64);
-        return __builtin_amdgcn_readfirstlane(__shfl(over ? first : some, from, 64));
+        base = from_lane(over ? at_first : at_some, from);
+        return from_lane(over ? first : some, from);
     }
 };
 
@@ -260,9 +241,7 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
                     double x[8], mine = 0.0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) { x[j] = c + j < to ? w.at(c + j) : 0.0; mine += x[j]; }
-                    double incl = mine;
-#pragma unroll
-                    for (int o = 1; o < 64; o <<= 1) { const double y = __shfl_up(incl, o, 64); if (lane >= o) incl += y; }
+                    const double incl = wave_scan(mine);
                     double run = base + (incl - mine);
                     int64_t first = -1, some = -1;
 #pragma unroll
@@ -271,9 +250,9 @@ __global__ __launch_bounds__(64 * NW) void verify_kernel(VerifyArgs a) {
                         if (x[j] > 0.0) { some = c + j; if (run > t && first < 0) first = c + j; }
                     }
                     const unsigned long long over = __ballot(first >= 0), with = __ballot(some >= 0);
-                    if (over) { word = __shfl(first, __builtin_ctzll(over), 64); break; }
-                    if (with) word = __shfl(some, 63 - __builtin_clzll(with), 64);        // the last with weight, should roundings leave none over t
-                    base += __shfl(incl, 63, 64);
+                    if (over) { word = from_lane(first, __builtin_ctzll(over)); break; }
+                    if (with) word = from_lane(some, 63 - __builtin_clzll(with));        // the last with weight, should roundings leave none over t
+                    base += from_lane(incl, 63);
                 }
             }
             break;
