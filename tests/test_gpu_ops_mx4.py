@@ -246,3 +246,31 @@ def test_captured_and_replayed(ops, m):
         torch.cuda.synchronize()
         want = ops.mx4_linear(x, w)
         assert torch.equal(y, want) and torch.equal(z, ops.mx4_dequantize(ops.mx4_quantize(want)))
+
+
+def test_offsets_past_32_bits(ops):
+    """2^20 + 5 rows of 8192: values, codes and results that lie more than 2^32 bytes or elements behind the first.  Values -1, 0, 1 are
+    exact in the form, sums of 8192 products of them are whole numbers under 2^24."""
+    rows, k = 2 ** 20 + 5, 8192
+    x = torch.randint(-1, 2, (rows, k), dtype=torch.int8, device=DEV).to(torch.bfloat16)
+    q = ops.mx4_quantize(x)
+    assert x.numel() > 2 ** 32 and q.codes.numel() > 2 ** 32
+    back = ops.mx4_dequantize(q, torch.bfloat16)
+    assert all(torch.equal(back[r:r + 65536], x[r:r + 65536]) for r in range(0, rows, 65536))
+    del back
+    ends = torch.cat([torch.arange(7), torch.arange(rows // 2 - 3, rows // 2 + 3), torch.arange(rows - 40, rows)]).to(DEV)
+    few = x[rows // 3:rows // 3 + 4].float()
+    want = few.double() @ x[ends].double().t()
+    assert torch.equal(ops.mx4_linear(few, q)[:, ends].double(), want)                  # one launch
+    many = few.repeat(25, 1)
+    assert torch.equal(ops.mx4_linear(many, q)[:, ends].double(), want.repeat(25, 1))   # two launches, w past 32 bits
+    right = x[1000:4000].float()
+    y = ops.mx4_matmul(q, ops.mx4_quantize(right))                                      # y past 32 bits
+    assert y.numel() * 4 > 2 ** 33
+    assert torch.equal(y[ends].double(), x[ends].double() @ right.double().t())
+    del y
+    tall = x[:, :4100].t()                                                              # (4100, rows): rows neighbours in memory
+    qt = ops.mx4_quantize(tall[:, rows - 70000:])
+    assert torch.equal(ops.mx4_dequantize(qt, torch.bfloat16), tall[:, rows - 70000:])
+    x = q = tall = qt = None
+    torch.cuda.empty_cache()

@@ -166,3 +166,16 @@ def test_captions_follow_the_target(ops):
     count = torch.bincount(words[:, 0].cpu(), minlength=v).double()
     e = n * p.double() / p.double().sum()
     assert float(((count - e) ** 2 / e).sum()) < 110 and 0 < float(acc.float().mean()) < 1
+
+
+def test_offsets_past_32_bits(ops):
+    """Captions 2^31 + 24 elements apart."""
+    d, t, p, au, du = make(3, 2, 1000, torch.bfloat16, 21)
+    step = 2 ** 31 + 24
+    far = torch.empty(2 * step + 3000, dtype=torch.bfloat16, device=DEV)
+    ft, fp = far.as_strided((3, 3, 1000), (step, 1000, 1)), torch.empty_like(far).as_strided((3, 2, 1000), (step, 1000, 1))
+    ft.copy_(t)
+    fp.copy_(p)
+    check(ops, [d, ft, fp, au, du])
+    far = ft = fp = None
+    torch.cuda.empty_cache()
