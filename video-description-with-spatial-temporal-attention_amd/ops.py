@@ -7,8 +7,13 @@ next-word distribution -- the pieces of `Decoder.sample_drafted`, for programs t
 
 Every call forwards to one entry point of include/stattn.h, which states what is computed.  Work is enqueued on the current stream of
 the tensors' device (which need not be the current device); results are new tensors.  Arguments of a wrong type raise TypeError, of a
-wrong size or place ValueError; there is no CPU fallback."""
+wrong size or place ValueError; there is no CPU fallback.
+
+These are operators of decoding: none has a gradient.  A product of tensors that record one (x or bias with requires_grad, outside
+torch.no_grad()) is computed all the same, and its backward raises RuntimeError; forward-mode tangents raise at the call.  The 4-bit form
+and the words of verify_draft are whole numbers, through which nothing is differentiated, as through any cast to integers in torch."""
 import torch
+from torch.autograd import forward_ad
 
 try:
     from . import _native
@@ -38,6 +43,25 @@ def _wrong_place(dev, **tensors):
     for name, t in tensors.items():
         if t is not None and t.get_device() != dev:
             raise ValueError("%s is on %s, not on cuda:%d" % (name, t.device, dev))
+
+
+class _NoGradient(torch.autograd.Function):
+    """`y` as it is, on the record of the tensors it was computed from: a backward pass through it fails instead of leaving them out."""
+
+    @staticmethod
+    def forward(ctx, y, name, *inputs):
+        ctx.name = name
+        return y
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % ctx.name)
+
+
+def _tangent(name, *tensors):
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("%s has no derivative (an argument carries a forward-mode tangent)" % name)
 
 
 class MX4(object):
@@ -141,11 +165,15 @@ def mx4_matmul(a, w, bias=None, dtype=torch.float32):
         _wrong_place(dev, a_scales=as_, w=wc, w_scales=ws)
     m, n = ac.shape[0], wc.shape[0]
     b = None if bias is None else _check_bias(bias, n, dev)
+    if forward_ad._current_level >= 0:
+        _tangent("mx4_matmul", bias)
     y = ac.new_empty((m, n), dtype=dtype)
     rc = _native.load_library().stattn_mx4_matmul(dev, _raw_stream(dev), ac.data_ptr(), as_.data_ptr(), wc.data_ptr(), ws.data_ptr(), m, n, k, b,
                                                   y.data_ptr(), t, n)
     if rc:
         _fail(rc)
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        return _NoGradient.apply(y, "mx4_matmul", bias)
     return y
 
 
@@ -170,6 +198,8 @@ def mx4_linear(x, w, bias=None):
         _wrong_place(dev, w=wc, w_scales=ws)
     n = wc.shape[0]
     b = None if bias is None else _check_bias(bias, n, dev)
+    if forward_ad._current_level >= 0:
+        _tangent("mx4_linear", x, bias)
     lib = _native.load_library()
     y = x.new_empty((m, n))
     need = lib.stattn_mx4_linear_workspace(m, n, k)
@@ -178,6 +208,8 @@ def mx4_linear(x, w, bias=None):
                                work.data_ptr() if need else None, need)
     if rc:
         _fail(rc)
+    if (x.requires_grad or bias is not None and bias.requires_grad) and torch.is_grad_enabled():
+        return _NoGradient.apply(y, "mx4_linear", x, bias)
     return y
 
 
