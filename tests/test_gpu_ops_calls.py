@@ -53,3 +53,32 @@ def test_a_forward_mode_tangent_is_refused(ops):
         with pytest.raises(RuntimeError, match="mx4_matmul has no derivative"):
             ops.mx4_matmul(q, w, bias=dual)
     assert torch.equal(ops.mx4_linear(x, w, bias=bias), want)
+
+
+def lazy(t):
+    """The same numbers, their sign kept beside the memory."""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+def test_views_whose_sign_is_kept_beside_the_memory(ops):
+    z = torch.randn(40, 70, 2, device=DEV)
+    v = torch.view_as_complex(z).conj().imag                               # column stride 2
+    assert v.is_neg()
+    for axis in (0, 1):
+        got, want = ops.mx4_quantize(v, axis=axis), ops.mx4_quantize(-z[:, :, 1], axis=axis)
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    x, bias = torch.randn(40, 70, device=DEV), torch.randn(30, device=DEV)
+    w = ops.mx4_quantize(torch.randn(30, 70, device=DEV))
+    want, q = ops.mx4_linear(x, w, bias=bias), ops.mx4_quantize(x)
+    assert torch.equal(ops.mx4_linear(lazy(x), w, bias=bias), want) and torch.equal(ops.mx4_linear(x, w, bias=lazy(bias)), want)
+    assert torch.equal(ops.mx4_linear(lazy(x)[3:, :], w, bias=bias), want[3:])
+    assert torch.equal(ops.mx4_matmul(q, w, bias=lazy(bias)), ops.mx4_matmul(q, w, bias=bias))
+    g = torch.Generator().manual_seed(1)
+    t, p = (torch.softmax(3 * torch.randn(6, 3, 90, generator=g), 2).to(DEV) for _ in range(2))
+    args = [torch.randint(0, 90, (6, 2), generator=g).to(DEV), t, p[:, :2].contiguous(), torch.rand(6, 2, generator=g).to(DEV), torch.rand(6, generator=g).to(DEV)]
+    want = ops.verify_draft(*args)
+    for i in range(1, 5):
+        got = ops.verify_draft(*args[:i], lazy(args[i]), *args[i + 1:])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i

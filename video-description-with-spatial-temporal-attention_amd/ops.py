@@ -7,7 +7,8 @@ next-word distribution -- the pieces of `Decoder.sample_drafted`, for programs t
 
 Every call forwards to one entry point of include/stattn.h, which states what is computed.  Work is enqueued on the current stream of
 the tensors' device (which need not be the current device); results are new tensors.  Arguments of a wrong type raise TypeError, of a
-wrong size or place ValueError; there is no CPU fallback.
+wrong size or place ValueError; there is no CPU fallback.  A view whose sign torch keeps beside the memory (is_neg(): z.conj().imag) is
+written out first.
 
 These are operators of decoding: none has a gradient.  A product of tensors that record one (x or bias with requires_grad, outside
 torch.no_grad()) is computed all the same, and its backward raises RuntimeError; forward-mode tangents raise at the call.  The 4-bit form
@@ -109,6 +110,8 @@ def mx4_quantize(x, axis=-1):
         raise ValueError("x must have two dimensions")
     if axis not in (-2, -1, 0, 1):
         raise ValueError("axis must be 0 or 1")
+    if x.is_neg():
+        x = x.resolve_neg()
     dev = x.get_device()
     if dev < 0:
         _wrong_place(dev)
@@ -148,7 +151,7 @@ def _check_bias(bias, n, dev):
         raise ValueError("bias must be a contiguous vector of %d values" % n)
     if bias.get_device() != dev:
         _wrong_place(dev, bias=bias)
-    return bias.data_ptr()
+    return bias.resolve_neg()           # itself, unless is_neg()
 
 
 def mx4_matmul(a, w, bias=None, dtype=torch.float32):
@@ -164,12 +167,13 @@ def mx4_matmul(a, w, bias=None, dtype=torch.float32):
     if dev < 0 or as_.get_device() != dev or wc.get_device() != dev or ws.get_device() != dev:
         _wrong_place(dev, a_scales=as_, w=wc, w_scales=ws)
     m, n = ac.shape[0], wc.shape[0]
-    b = None if bias is None else _check_bias(bias, n, dev)
+    if bias is not None:
+        bias = _check_bias(bias, n, dev)
     if forward_ad._current_level >= 0:
         _tangent("mx4_matmul", bias)
     y = ac.new_empty((m, n), dtype=dtype)
-    rc = _native.load_library().stattn_mx4_matmul(dev, _raw_stream(dev), ac.data_ptr(), as_.data_ptr(), wc.data_ptr(), ws.data_ptr(), m, n, k, b,
-                                                  y.data_ptr(), t, n)
+    rc = _native.load_library().stattn_mx4_matmul(dev, _raw_stream(dev), ac.data_ptr(), as_.data_ptr(), wc.data_ptr(), ws.data_ptr(), m, n, k,
+                                                  None if bias is None else bias.data_ptr(), y.data_ptr(), t, n)
     if rc:
         _fail(rc)
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():
@@ -186,6 +190,8 @@ def mx4_linear(x, w, bias=None):
     shape, k = x.shape, w.cols
     if len(shape) != 2 or shape[1] != k:
         raise ValueError("x must be (m, %d), got %s" % (k, tuple(shape)))
+    if x.is_neg():
+        x = x.resolve_neg()
     m = shape[0]
     ld, one = x.stride()
     if m <= 1:
@@ -197,15 +203,16 @@ def mx4_linear(x, w, bias=None):
     if dev < 0 or wc.get_device() != dev or ws.get_device() != dev:
         _wrong_place(dev, w=wc, w_scales=ws)
     n = wc.shape[0]
-    b = None if bias is None else _check_bias(bias, n, dev)
+    if bias is not None:
+        bias = _check_bias(bias, n, dev)
     if forward_ad._current_level >= 0:
         _tangent("mx4_linear", x, bias)
     lib = _native.load_library()
     y = x.new_empty((m, n))
     need = lib.stattn_mx4_linear_workspace(m, n, k)
     work = x.new_empty((need,), dtype=_U8) if need else None        # alive until the launches are enqueued
-    rc = lib.stattn_mx4_linear(dev, _raw_stream(dev), x.data_ptr(), dtype, ld, wc.data_ptr(), ws.data_ptr(), m, n, k, b, y.data_ptr(), n,
-                               work.data_ptr() if need else None, need)
+    rc = lib.stattn_mx4_linear(dev, _raw_stream(dev), x.data_ptr(), dtype, ld, wc.data_ptr(), ws.data_ptr(), m, n, k,
+                               None if bias is None else bias.data_ptr(), y.data_ptr(), n, work.data_ptr() if need else None, need)
     if rc:
         _fail(rc)
     if (x.requires_grad or bias is not None and bias.requires_grad) and torch.is_grad_enabled():
@@ -230,6 +237,8 @@ def verify_draft(draft, target, proposal, accept_u, draw_u, lens=None):
         raise TypeError("draft must be int64, accept_u and draw_u float32")
     if draft.shape != (b, j) or accept_u.shape != (b, j) or draw_u.shape != (b,):
         raise ValueError("draft and accept_u must be (%d, %d), draw_u (%d,)" % (b, j, b))
+    if target.is_neg() or accept_u.is_neg() or draw_u.is_neg():
+        target, accept_u, draw_u = target.resolve_neg(), accept_u.resolve_neg(), draw_u.resolve_neg()
     tb, tj, tv = target.stride()
     db, dj = draft.stride()
     ub, uj = accept_u.stride()
@@ -241,6 +250,8 @@ def verify_draft(draft, target, proposal, accept_u, draw_u, lens=None):
     if proposal is not None:
         if proposal.dtype != target.dtype:
             raise TypeError("proposal must have target's type (%s), got %s" % (target.dtype, proposal.dtype))
+        if proposal.is_neg():
+            proposal = proposal.resolve_neg()
         pb, pj, pv = proposal.stride() if proposal.dim() == 3 else (0, 0, 0)
         if proposal.shape != (b, j, v) or (v > 1 and pv != 1):
             raise ValueError("proposal must be (%d, %d, %d) with contiguous words" % (b, j, v))
