@@ -174,7 +174,8 @@ int stattn_sample_search(stattn_handle* h, int nvid, const float* ctxg, const fl
  * sample of those, plus one word drawn from them.  Between 1 and draft + 1 words a round, whatever the 4-bit copy is worth.
  * 1 <= nvid <= 16, 1 <= maxlen <= 65536; features as in stattn_sample_search; every precision.  `uniforms`: the numbers in [0, 1) that decide, host memory
  * (maxlen, 2 * draft + 1, nvid) -- a round takes one row each for the draws of its drafts, for their checks and for the last word --
- * or NULL: from the handle's seed and a per-call counter.  out_drafted / out_kept (nvid) or NULL: words drafted and kept, a caption. */
+ * or NULL: from the handle's seed and a per-call counter.  out_drafted / out_kept (nvid) or NULL: the words drafted for a caption and those
+ * the check kept, whole rounds: every round of it counts `draft` words drafted, and kept words behind its end (<eos>, maxlen) count too. */
 int stattn_sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl,
                           const float* ctxm, int T, int K, int draft, int maxlen, const float* uniforms,
                           int64_t* out_tokens, float* out_scores, int32_t* out_lens, int32_t* out_drafted, int32_t* out_kept);

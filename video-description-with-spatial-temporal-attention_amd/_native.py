@@ -534,9 +534,10 @@ class Decoder(object):
 
     def sample_drafted(self, ctxg=None, ctxg_mask=None, ctxl=None, ctxm=None, draft=4, maxlen=30, resident=False, uniforms=None):
         """sample_search with the vocabulary projection out of the word loop (stattn_sample_drafted): a 4-bit copy of it drafts `draft`
-        words at a time and the full-precision one checks them together.  The same return value, drawn from the same distributions; the
-        words drafted and kept of each caption are in `self.draft_counts`, two int32 vectors.  `uniforms` (maxlen, 2 * draft + 1, nvid)
-        float32 in [0, 1) makes the draws the caller's."""
+        words at a time and the full-precision one checks them together.  The same return value, drawn from the same distributions.
+        `self.draft_counts`, two int32 vectors: the words drafted for each caption and those the check kept, whole rounds -- a round
+        counts `draft` words drafted, and words kept behind the caption's end (its <eos>, maxlen) as well.  `uniforms`
+        (maxlen, 2 * draft + 1, nvid) float32 in [0, 1) makes the draws the caller's."""
         if resident:
             if getattr(self, "_staged", None) is None:
                 raise ValueError("sample_drafted(resident=True) needs beam_stage() first")

@@ -596,13 +596,16 @@ class Attention(object):
     def gen_sample_drafted(self, tparams, options, ctxgs, ctxg_masks, ctxls, ctxms, draft=4, maxlen=30, uniforms=None):
         """gen_sample(stochastic=True) (model_attention.py:863-918) for a batch of videos, with words drafted by a 4-bit copy of the
         vocabulary projection and checked by the full-precision one, several at a time (Decoder.sample_drafted): [(sample, score), ...]
-        per video, samples of the same distributions.  Any number of videos; sixteen go through the device together."""
+        per video, samples of the same distributions.  Any number of videos; sixteen go through the device together.  The words drafted
+        and kept of each video are then in the decoder's `draft_counts`."""
         dec = self._bind(tparams, options)
-        out = []
+        out, counts = [], [numpy.zeros((2, 0), numpy.int32)]
         for v in range(0, len(ctxgs), 16):
             part = slice(v, v + 16)
             u = None if uniforms is None else numpy.ascontiguousarray(uniforms[:, :, part])
             out += dec.sample_drafted(ctxgs[part], ctxg_masks[part], ctxls[part], ctxms[part], draft=draft, maxlen=maxlen, uniforms=u)
+            counts.append(numpy.stack(dec.draft_counts))
+        dec.draft_counts = tuple(numpy.concatenate(counts, 1))
         return out
 
     # ---------------------------------------------------------------- teacher-forced scoring
