@@ -31,7 +31,7 @@ template <OpType T>
 __global__ __launch_bounds__(256) void mx4_quantize_cols_kernel(Mx4QuantArgs a, unsigned row_tiles, unsigned kp128) {
     typedef typename Elem<T>::type E;
     __shared__ uint4 code[64][5];                    // a row's four blocks, one slot apart from the next row's banks
-    __shared__ uint8_t scale[64][4];
+    __shared__ unsigned scale[64];                   // a row's four scale bytes
     const int lane = threadIdx.x & 63, blk = threadIdx.x >> 6;
     for (int64_t t = blockIdx.x; t < (int64_t)row_tiles * kp128; t += gridDim.x) {
         const int64_t r0 = t % row_tiles * 64, c0 = t / row_tiles * 128, r = r0 + lane, c = c0 + blk * 32;
@@ -47,13 +47,13 @@ __global__ __launch_bounds__(256) void mx4_quantize_cols_kernel(Mx4QuantArgs a, 
         }
         const unsigned byte = mx4_scale_byte(max(max(top8(v), top8(v + 8)), max(top8(v + 16), top8(v + 24))));
         code[lane][blk] = make_uint4(mx4_codes8(v, byte), mx4_codes8(v + 8, byte), mx4_codes8(v + 16, byte), mx4_codes8(v + 24, byte));
-        scale[lane][blk] = (uint8_t)byte;
+        reinterpret_cast<uint8_t*>(&scale[lane])[blk] = (uint8_t)byte;
         __syncthreads();
         const int64_t ro = r0 + (threadIdx.x >> 2);
         if (ro < a.rows) {
             const int64_t at = ro * kp128 * 4 + c0 / 32;
             reinterpret_cast<uint4*>(a.codes)[at + (threadIdx.x & 3)] = code[threadIdx.x >> 2][threadIdx.x & 3];
-            if ((threadIdx.x & 3) == 0) *reinterpret_cast<unsigned*>(a.scales + at) = *reinterpret_cast<const unsigned*>(scale[threadIdx.x >> 2]);
+            if ((threadIdx.x & 3) == 0) *reinterpret_cast<unsigned*>(a.scales + at) = scale[threadIdx.x >> 2];
         }
         __syncthreads();
     }
