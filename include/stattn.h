@@ -303,12 +303,14 @@ int stattn_mx4_quantize(int device, void* stream, const void* x_dev, int dtype, 
 int stattn_mx4_dequantize(int device, void* stream, const void* codes_dev, const void* scales_dev, int64_t rows, int64_t cols,
                           void* out_dev, int dtype, int64_t ld_out);
 /* y[i][j] = sum_c a[i][c] w[j][c] + bias[j]: a (m, k) and w (n, k) in the 4-bit form, bias float32 or NULL, y (m, n) of type `dtype`
- * with row stride ld_y (n <= ld_y < 2^22).  Products are exact, sums are in fp32, rounded once to the type. */
+ * with row stride ld_y (n <= ld_y < 2^22).  A product is exact where fp32 holds it (infinite beyond 2^128, a multiple of 2^-149 under 2^-126),
+ * sums are in fp32 in any order, rounded once to the type. */
 int stattn_mx4_matmul(int device, void* stream, const void* a_codes_dev, const void* a_scales_dev, const void* w_codes_dev,
                       const void* w_scales_dev, int64_t m, int64_t n, int64_t k, const float* bias_dev,
                       void* y_dev, int dtype, int64_t ld_y);
-/* The same with a = x (m, k) of type `dtype`, row stride ld_x, brought into the 4-bit form on the way: the result is that of
- * stattn_mx4_quantize followed by stattn_mx4_matmul.  y is of x's type.  `workspace_dev`: stattn_mx4_linear_workspace(m, n, k) bytes,
+/* The same with a = x (m, k) of type `dtype`, row stride ld_x, brought into the 4-bit form on the way: the codes are those of
+ * stattn_mx4_quantize, the result that of a stattn_mx4_matmul behind it up to the order of the sums, which goes by m and k: a row's
+ * last bits may differ between calls of different m.  y is of x's type.  `workspace_dev`: stattn_mx4_linear_workspace(m, n, k) bytes,
  * 16-byte aligned, overwritten (may be NULL when that is 0); not to be shared by calls that can run at the same time. */
 size_t stattn_mx4_linear_workspace(int64_t m, int64_t n, int64_t k);
 int stattn_mx4_linear(int device, void* stream, const void* x_dev, int dtype, int64_t ld_x, const void* w_codes_dev,
