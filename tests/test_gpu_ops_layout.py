@@ -112,3 +112,21 @@ def test_check_in_a_frame(ops, lib, b, j, v):
     want = ops.verify_draft(d, t, p, au, du)
     assert torch.equal(words, want[0]) and torch.equal(acc[:b], want[1])
     assert untouched(big, words, 99) and bool((acc[b:] == 99).all()) and bool((work[need:] == 9).all())
+
+
+@pytest.mark.parametrize("dtype,code", TYPES[:2])
+def test_the_largest_row_stride(ops, lib, dtype, code):
+    """Row strides of 2^22 - 1 elements, the largest that is accepted: the last row of a 256-row tile in fp32 ends just under 2^32 bytes
+    behind its first.  Between the rows, and in the columns beside the result, nothing is written."""
+    m, n, k, ld = 2047, 4095, 1030, 2 ** 22 - 1
+    assert tile(m, n, k) == 256
+    a, w = ops.mx4_quantize(torch.randn(m, k, device=DEV)), ops.mx4_quantize(torch.randn(n, k, device=DEV))
+    big = torch.full((m + 1, ld), 7, dtype=dtype, device=DEV)
+    y = big[:m, 5:5 + n]
+    assert lib.stattn_mx4_matmul(0, stream(), a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), m, n, k, None,
+                                 y.data_ptr(), code, ld) == 0
+    assert torch.equal(y, ops.mx4_matmul(a, w, dtype=dtype))
+    y.fill_(7)
+    assert all(bool((big[r:r + 64] == 7).all()) for r in range(0, m + 1, 64))
+    big = y = None
+    torch.cuda.empty_cache()
