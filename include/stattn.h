@@ -326,7 +326,8 @@ int stattn_mx4_linear(int device, void* stream, const void* x_dev, int dtype, in
  * first whose running sum of weights exceeds draw_u * total, weights max(target - proposal, 0) at the refused position (target itself
  * if all of them are 0), or target behind a draft that was kept whole.  accepted[i] = kept words; words row i = the kept words, the
  * drawn one, -1 from there on.  The captions that result are samples of the target's distribution.  Products and sums are in 64 bits;
- * weights that are NaN count as 0; a drafted word outside [0, v) is refused; a row without any weight draws -1.
+ * weights that are NaN or negative count as 0; a drafted word outside [0, v) is refused; a row without any weight draws -1; where no
+ * running sum exceeds draw_u * total (infinite weights, numbers of 1 and more) the last word with weight is drawn.
  * `workspace_dev`: stattn_verify_draft_workspace(b, j, v) bytes, 16-byte aligned, overwritten (may be NULL when that is 0); not to be
  * shared by calls that can run at the same time. */
 size_t stattn_verify_draft_workspace(int64_t b, int64_t j, int64_t v);

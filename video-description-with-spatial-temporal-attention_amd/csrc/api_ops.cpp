@@ -87,7 +87,7 @@ static int product_ok(const char* who, int64_t m, int64_t n, int64_t k, const vo
     if (!type_ok(dtype)) return refuse(STATTN_EINVAL, "%s: dtype %d is none of STATTN_F32, STATTN_BF16, STATTN_F16", who, dtype);
     if (ld_y < n || ld_y >= (int64_t)1 << 22) return refuse(STATTN_EINVAL, "%s: ld_y (%lld) must be at least n (%lld) and under 2^22", who, (long long)ld_y, (long long)n);
     if (m && n && !y) return refuse(STATTN_EINVAL, "%s: null y", who);
-    // as many 32 x 32 tiles as a launch can hold workgroups
+    // the smallest tile is 64 x 64, so this keeps the workgroups of a launch under 2^22
     if ((m + 31) / 32 * ((n + 31) / 32) >= (int64_t)1 << 24) return refuse(STATTN_EINVAL, "%s: a product of %lld x %lld is too large for one call", who, (long long)m, (long long)n);
     (void)k;
     return STATTN_OK;
@@ -109,7 +109,8 @@ int stattn_mx4_matmul(int device, void* stream, const void* a_codes, const void*
 // Few rows: one launch in which every workgroup rounds x for itself, instead of two with x's 4-bit form between them.  Up to 32768
 // values of x that takes the GPU little longer (1 x 12000 x 512: 3.5 us against 5.1; 32: 6.0 against 5.6; 64: 9.1 against 5.8; beyond,
 // 64 x 20000 x 1024: 18.5 against 7.4) and saves the caller a launch and a workspace, 4.5 us of its time.  Rows whose last eight are
-// partial load one by one in between (64 x 12000 x 511: 12): up to 16384.
+// partial load one by one in between (64 x 12000 x 511: 12): up to 16384.  The rule is the eager caller's: replayed in a graph, where a
+// launch and a workspace cost nothing more, two launches are the faster way from about 32 rows of 512 on (64 x 12000 x 512: 9.1 against 5.8).
 static bool few_rows(int64_t m, int64_t k) { return m <= 64 && m * k <= (k % 8 ? 16384 : 32768); }
 
 size_t stattn_mx4_linear_workspace(int64_t m, int64_t n, int64_t k) {

@@ -1,9 +1,10 @@
 // Products of two matrices in microscaled 4 bits on the matrix cores: v_mfma_scale_f32_32x32x64_f8f6f4 multiplies 32 x 64 codes by
 // 64 x 32 codes under their block scales and adds in fp32.  Lane l of the wave holds row l % 32 and the block l / 32 of an operand:
 // exactly one 16-byte block of the row-major form and its scale byte, so operands go from memory to registers as they are.
-// 8192^3 in bf16: 253 .. 274 us (4.0 .. 4.3 PFLOP/s), 214 with all codes 0, 500 at K = 16384: the chip's power is what bounds long sums of
-// random codes (the clock falls to 1.85 GHz; the matrix pipe is busy 60% of it).  1920 x 12000 x 512 in fp32: 20 us, its 92 MB of y at
-// 4.8 TB/s.  Few tiles (64 x 1024 x 4096: 8.4 us): a round trip a stage.
+// 8192^3 in bf16: 257 .. 282 us (3.9 .. 4.3 PFLOP/s), 200 .. 211 with all codes 0, 490 .. 500 at K = 16384.  It takes 474000 cycles whatever the
+// codes, of which the matrix pipe is busy 55% (waves wait for 16%); random codes run them at 1.83 GHz, zeros at 2.36: the schedule and the
+// chip's power bound it together.  1920 x 12000 x 512 in fp32: 20 us, its 92 MB of y at 4.8 TB/s.  Few tiles (64 x 1024 x 4096: 8.4 us): a
+// round trip a stage.
 #include "mx4_inl.h"
 
 namespace stattn {

@@ -10,7 +10,7 @@ namespace stattn {
 enum OpType { OP_F32 = 0, OP_BF16 = 1, OP_F16 = 2 };
 
 // The 4-bit form of a (rows, cols) matrix: codes [rows][kp / 2] bytes (even column in the low half), scales [rows][kp / 32] bytes,
-// kp = cols rounded up to 128.  Both pointers 16-byte aligned.
+// kp = cols rounded up to 128.  Codes are 16-byte, scales 4-byte aligned.
 struct Mx4View { const uint8_t* codes; const uint8_t* scales; int64_t rows; int64_t cols; };
 __host__ __device__ inline int64_t mx4_kp(int64_t cols) { return (cols + 127) / 128 * 128; }
 

@@ -224,7 +224,7 @@ def verify_draft(draft, target, proposal, accept_u, draw_u, lens=None):
     """(words, accepted) of b captions with up to j drafted words each (stattn_verify_draft): draft (b, j) int64, target (b, j + 1, v) and
     proposal (b, j, v) -- None for arg-max drafts -- probabilities of one floating type with contiguous words, accept_u (b, j) and
     draw_u (b,) float32 in [0, 1), lens (b,) int32 or None.  words (b, j + 1) int64: the kept words, the drawn one, then -1;
-    accepted (b,) int32: how many were kept."""
+    accepted (b,) int32: how many were kept.  (lens of another type or size: ValueError.)"""
     dtype = _DTYPE.get(target.dtype)
     if dtype is None:
         _wrong_type("target", target.dtype)
