@@ -87,7 +87,7 @@ static int sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
         for (size_t i = 0; i < nu; ++i) drawn[i] = (float)(mix(seed + 0x9E3779B97F4A7C15ull * (i + 1)) >> 40) * (1.0f / 16777216.0f);
         uniforms = drawn.data();
     }
-    HIPCHK(h, hipMemcpy(ub, uniforms, nu * sizeof(float), hipMemcpyHostToDevice));
+    HIPCHK(h, copy_now(s, ub, uniforms, nu * sizeof(float), hipMemcpyHostToDevice));
     HIPCHK(h, launch_mx4_quantize(s, Mx4QuantArgs{w.Wo, OP_F32, V, E, 1, Vp, hc, hsc}));      // ff_logit_W is (dim_word, n_words)
     HIPCHK(h, launch_iota(s, vid, M, 1));
     HIPCHK(h, launch_fill(s, dp, 0.5f, (size_t)M * 3 * D));                                  // use_noise = 0 (:469-472)
@@ -180,7 +180,7 @@ static int sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
     };
 
     // A round is some ten launches a word, each a few microseconds: captured once and replayed while the buffers and shapes stay the same.
-    // Falls back to plain launches if the capture is refused (and under profiling, whose events a graph would not time).
+    // Plain launches where that fails (and under profiling, whose events a graph would not time); the next call captures again.
     hipGraphExec_t ge = nullptr;
     std::vector<uintptr_t> sig = {(uintptr_t)nvid, (uintptr_t)T, (uintptr_t)K, (uintptr_t)draft, (uintptr_t)maxlen, (uintptr_t)panels, (uintptr_t)s};
     for (const void* b : {(const void*)c.G, (const void*)c.L, (const void*)c.Mo, (const void*)c.PG, (const void*)c.PL, (const void*)c.PM, (const void*)c.LW,
@@ -197,15 +197,7 @@ static int sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
             ge = h->draft_gexec;
         } else {
             if (h->draft_gexec) { (void)hipGraphExecDestroy(h->draft_gexec); h->draft_gexec = nullptr; }
-            hipGraph_t graph = nullptr;
-            bool ok = hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal) == hipSuccess;
-            if (ok) {
-                const int r = round();
-                const hipError_t e = hipStreamEndCapture(s, &graph);
-                ok = r == STATTN_OK && e == hipSuccess && graph && hipGraphInstantiate(&ge, graph, nullptr, nullptr, 0) == hipSuccess;
-            }
-            if (graph) (void)hipGraphDestroy(graph);
-            if (!ok) { ge = nullptr; (void)hipGetLastError(); }
+            ge = capture_graph(h, s, round);
             h->draft_gexec = ge; h->draft_gsig = sig;
         }
     }
@@ -219,7 +211,7 @@ static int sample_drafted(stattn_handle* h, int nvid, const float* ctxg, const f
         for (const DraftInfo& f : info) live = live || !f.done;
         if (!live) break;
     }
-    HIPCHK(h, hipMemcpy(out_tokens, d.tokens, (size_t)M * maxlen * sizeof(int64_t), hipMemcpyDeviceToHost));
+    HIPCHK(h, copy_now(s, out_tokens, d.tokens, (size_t)M * maxlen * sizeof(int64_t), hipMemcpyDeviceToHost));
     for (int m = 0; m < M; ++m) {
         out_scores[m] = info[m].score; out_lens[m] = info[m].len;
         if (out_drafted) out_drafted[m] = info[m].drafted;
