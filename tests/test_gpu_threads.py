@@ -1,5 +1,6 @@
-"""Searches on a handle while another thread uses the GPU.  On this runtime a copy through the legacy stream (hipMemcpy) or a
-hipDeviceSynchronize, made by any thread while a stream is being captured, fails, and the capture can be neither used nor ended."""
+"""Drafted sampling while another thread uses the GPU.  On this runtime a copy through the legacy stream (hipMemcpy) or a
+hipDeviceSynchronize, made by any thread while a stream is being captured, fails, and the capture can be neither used nor ended: so the
+call captures nothing."""
 import ctypes
 import threading
 
@@ -12,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 
 class LegacyCopies(object):
-    """A thread that copies through the legacy stream all the time; `failed` counts the copies that met a capture."""
+    """A thread that copies through the legacy stream all the time; `failed` counts the copies that were refused."""
 
     def __enter__(self):
         hip = ctypes.CDLL("libamdhip64.so")
@@ -35,9 +36,8 @@ class LegacyCopies(object):
         self.thread.join()
 
 
-def test_drafted_sampling_survives_an_interrupted_capture(stattn_mod, O):      # noqa: F811
-    """Thirty calls of different shapes, each of which captures its launches: the results are those of an undisturbed handle, and the handle
-    works on, captures included, when the other thread has stopped."""
+def test_drafted_sampling_beside_another_threads_copies(stattn_mod, O):      # noqa: F811
+    """Thirty calls of different shapes: no copy of the other thread fails, and the results are those of an undisturbed handle."""
     opt, P = small(O)
     b = O.synthetic_batch(opt, B=3, T=5, K=3, t=3, seed=81)
 
@@ -48,6 +48,5 @@ def test_drafted_sampling_survives_an_interrupted_capture(stattn_mod, O):      #
     want = [call(quiet, n) for n in range(1, 31)]
     with LegacyCopies() as other:
         got = [call(dec, n) for n in range(1, 31)]
-    assert other.failed > 0 and other.copies > 0
     assert got == want
-    assert [call(dec, n) for n in range(1, 31)] == want
+    assert other.copies > 30 and other.failed == 0

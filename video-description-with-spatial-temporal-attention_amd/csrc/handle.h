@@ -138,10 +138,6 @@ struct stattn_handle {
     hipGraphExec_t beam_gexec_last = nullptr;   // two words, the second one the LAST of a search (no attention launch for a word that never comes)
     hipGraphExec_t beam_gexec8 = nullptr;   // eight words: a replay costs 10-16 us of launch overhead whatever it holds
     std::vector<uintptr_t> beam_gsig;
-    // drafted sampling: one round (all launches between two looks at the captions), kept the same way
-    hipStream_t capture_stream = nullptr;       // what capture_graph records on
-    hipGraphExec_t draft_gexec = nullptr;
-    std::vector<uintptr_t> draft_gsig;
     long beam_graph_replays = 0;        // replays in the last stattn_beam_search (0 = eager launches)
     // which code path the decoder steps took (stattn_dbg_counter 1..4; reset by stattn_forward_train / stattn_backward):
     // forward steps whose attention launch carried the h.U rider, forward steps on the row-panel kernels, reverse steps
@@ -237,39 +233,11 @@ inline float* findbuf(stattn_handle* h, const char* name) {
     return it == h->bufs.end() ? nullptr : static_cast<float*>(it->second.p);
 }
 
-// A copy between host and device memory on stream `s`, waited for.  hipMemcpy would go through the legacy stream: while any thread captures a
-// stream it fails, and that capture is lost.
+// A copy between host and device memory on stream `s`, waited for.  (hipMemcpy goes through the legacy stream: while any thread of the
+// process captures a stream, it fails, and that capture is lost.)
 inline hipError_t copy_now(hipStream_t s, void* dst, const void* src, size_t bytes, hipMemcpyKind kind) {
     const hipError_t e = hipMemcpyAsync(dst, src, bytes, kind, s);
     return e != hipSuccess ? e : hipStreamSynchronize(s);
-}
-
-// What `work` (an int(), a STATTN_* code) enqueues on the handle's stream, as a graph; null if it fails or the capture does, and then the
-// caller launches plainly.  `s` is the caller's name for that stream.  It is recorded on a stream of its own: another thread's
-// hipDeviceSynchronize or copy through the legacy stream invalidates a capture, and such a stream can do nothing but be destroyed.
-template <class F>
-inline hipGraphExec_t capture_graph(stattn_handle* h, hipStream_t& s, F work) {
-    struct Recording {
-        stattn_handle* h; hipStream_t& s; hipStream_t mine; bool ended = false;
-        ~Recording() {
-            h->stream = s = mine;
-            if (!ended) { (void)hipStreamDestroy(h->capture_stream); h->capture_stream = nullptr; (void)hipGetLastError(); }
-        }
-    };
-    hipGraph_t graph = nullptr;
-    hipGraphExec_t exec = nullptr;
-    if (!h->capture_stream && hipStreamCreateWithFlags(&h->capture_stream, hipStreamNonBlocking) != hipSuccess) { h->capture_stream = nullptr; (void)hipGetLastError(); return nullptr; }
-    {
-        Recording r{h, s, h->stream};
-        if (hipStreamBeginCapture(h->capture_stream, hipStreamCaptureModeThreadLocal) != hipSuccess) return nullptr;
-        h->stream = s = h->capture_stream;
-        const int rc = work();
-        r.ended = hipStreamEndCapture(h->capture_stream, &graph) == hipSuccess;
-        if (r.ended && rc == STATTN_OK && graph && hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0) != hipSuccess) exec = nullptr;
-    }
-    if (graph) (void)hipGraphDestroy(graph);
-    if (!exec) (void)hipGetLastError();
-    return exec;
 }
 
 // The regions of the flat gradient buffer in the order stattn_backward completes them (api_backward.cpp region_done), each

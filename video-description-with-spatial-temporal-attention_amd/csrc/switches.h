@@ -21,7 +21,7 @@ namespace stattn {
     X(STATTN_GEMM_NOGROUP)     /* one launch per GEMM problem instead of grouped launches                  tests/test_gpu_z3_switches.py, bench.py accounting */ \
     X(STATTN_READOUT_NOPAIR)   /* readout as two GEMMs instead of one K-concatenated launch                tests/test_gpu_z3_switches.py */ \
     X(STATTN_WIDE_STATS_FROM)  /* first beam width whose vocabulary launch uses the wide statistics path   tests/test_gpu_z3_switches.py (65 = stored logits) */ \
-    X(STATTN_BEAM_NOGRAPH)     /* stattn_beam_search and stattn_sample_drafted without hipGraph capture   tests/test_gpu_z3_switches.py, test_gpu_sample_drafted.py */ \
+    X(STATTN_BEAM_NOGRAPH)     /* word loop of stattn_beam_search without hipGraph capture                 tests/test_gpu_z3_switches.py */ \
     X(STATTN_COMM_NO_OVERLAP)  /* one all-reduce after the backward pass instead of five overlapped ones   fallback, tests/test_gpu_dp2.py */ \
     X(STATTN_DBG_REDZONE)      /* canary zones around every device buffer, checked after every API call    tests/test_gpu_z1_redzone.py */
 
