@@ -149,7 +149,10 @@ int stattn_set_video(stattn_handle* h, const float* ctxg, const float* ctxl, con
  * suppress_eos != 0 forbids word 0 so that every hypothesis runs maxlen steps (benchmarks).
  * Host features are staged on every call; with ctxg = ctxg_mask = ctxl = ctxm = NULL the videos staged by
  * stattn_beam_stage (same nvid, T, K) are decoded (inputs resident in HBM: benchmarks, re-decoding after an
- * update).  k = 1 is gen_sample's greedy mode (arg-max word, :896-918 with stochastic=False). */
+ * update).  k = 1 is gen_sample's greedy mode (arg-max word, :896-918 with stochastic=False).
+ * The first search of a shape captures its words (this call and stattn_sample_search).  A stream capture allows no thread of the process a
+ * copy through the legacy stream or a hipDeviceSynchronize: such a call fails then, and the capturing handle is lost.  The library itself
+ * makes none, whatever its handles do at the same time; programs whose other threads do set STATTN_BEAM_NOGRAPH in the environment. */
 int stattn_beam_stage(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl,
                       const float* ctxm, int T, int K);
 int stattn_beam_search(stattn_handle* h, int nvid, const float* ctxg, const float* ctxg_mask, const float* ctxl,

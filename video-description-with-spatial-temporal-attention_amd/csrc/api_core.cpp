@@ -229,11 +229,12 @@ static int param_copy(stattn_handle* h, float* base, const char* name, float* ho
     HIPCHK(h, hipStreamSynchronize(h->stream));
     if (p.ndim == 2 && p.ld != (int)p.dims[1]) {   // padded rows (ff_logit_W)
         const size_t wbytes = (size_t)p.dims[1] * sizeof(float);
-        if (host_src) HIPCHK(h, hipMemcpy2D(dev, (size_t)p.ld * sizeof(float), host_src, wbytes, wbytes, (size_t)p.dims[0], hipMemcpyHostToDevice));
-        else HIPCHK(h, hipMemcpy2D(host_dst, wbytes, dev, (size_t)p.ld * sizeof(float), wbytes, (size_t)p.dims[0], hipMemcpyDeviceToHost));
+        if (host_src) HIPCHK(h, hipMemcpy2DAsync(dev, (size_t)p.ld * sizeof(float), host_src, wbytes, wbytes, (size_t)p.dims[0], hipMemcpyHostToDevice, h->stream));
+        else HIPCHK(h, hipMemcpy2DAsync(host_dst, wbytes, dev, (size_t)p.ld * sizeof(float), wbytes, (size_t)p.dims[0], hipMemcpyDeviceToHost, h->stream));
+        HIPCHK(h, hipStreamSynchronize(h->stream));
     } else {
-        if (host_src) HIPCHK(h, hipMemcpy(dev, host_src, n * sizeof(float), hipMemcpyHostToDevice));
-        else HIPCHK(h, hipMemcpy(host_dst, dev, n * sizeof(float), hipMemcpyDeviceToHost));
+        if (host_src) HIPCHK(h, copy_now(h->stream, dev, host_src, n * sizeof(float), hipMemcpyHostToDevice));
+        else HIPCHK(h, copy_now(h->stream, host_dst, dev, n * sizeof(float), hipMemcpyDeviceToHost));
     }
     return STATTN_OK;
 }
@@ -288,9 +289,9 @@ int stattn_set_dropout_masks(stattn_handle* h, const float* dp, const float* d1,
     CHK(getbuf_t(h, "dp", n_dp, &b_dp));
     CHK(getbuf_t(h, "d1", n_d1, &b_d1));
     CHK(getbuf_t(h, "d2", n_d2, &b_d2));
-    HIPCHK(h, hipMemcpy(b_dp, dp, n_dp * sizeof(float), hipMemcpyHostToDevice));
-    HIPCHK(h, hipMemcpy(b_d1, d1, n_d1 * sizeof(float), hipMemcpyHostToDevice));
-    HIPCHK(h, hipMemcpy(b_d2, d2, n_d2 * sizeof(float), hipMemcpyHostToDevice));
+    HIPCHK(h, copy_now(h->stream, b_dp, dp, n_dp * sizeof(float), hipMemcpyHostToDevice));
+    HIPCHK(h, copy_now(h->stream, b_d1, d1, n_d1 * sizeof(float), hipMemcpyHostToDevice));
+    HIPCHK(h, copy_now(h->stream, b_d2, d2, n_d2 * sizeof(float), hipMemcpyHostToDevice));
     h->masks_user = true; h->masks_t = t; h->masks_m = m; h->masks_state = 0;
     return STATTN_OK;
 }

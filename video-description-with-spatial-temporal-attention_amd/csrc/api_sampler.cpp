@@ -211,7 +211,7 @@ int stattn_f_next(stattn_handle* h, const int64_t* x, int m, const float* ctxg, 
                 out_sample[r] = pick;
             }
         } else {
-            HIPCHK(h, hipMemcpy(out_sample, dargmax, (size_t)m * sizeof(int64_t), hipMemcpyDeviceToHost));
+            HIPCHK(h, copy_now(s, out_sample, dargmax, (size_t)m * sizeof(int64_t), hipMemcpyDeviceToHost));
         }
     }
     return STATTN_OK;
@@ -360,7 +360,7 @@ static int beam_search_impl(stattn_handle* h, int nvid, const float* ctxg, const
     if (stochastic) {      // seed of this call's draws, in device memory (the captured word graph is reused from call to call)
         const unsigned long long draw_seed = (h->seed * 0x9E3779B97F4A7C15ull + 0x632BE59BD9B4E019ull * (++h->draw)) | 1ull;
         CHK(getbuf_t(h, "bs_seed", (size_t)1, &d_seed));
-        HIPCHK(h, hipMemcpy(d_seed, &draw_seed, sizeof draw_seed, hipMemcpyHostToDevice));
+        HIPCHK(h, copy_now(s, d_seed, &draw_seed, sizeof draw_seed, hipMemcpyHostToDevice));
     }
     float *proj = nullptr, *proj_step = nullptr, *ho_pk = nullptr, *vstats = nullptr;
     int vtile = 0;
