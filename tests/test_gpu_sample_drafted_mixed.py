@@ -1,5 +1,5 @@
-"""Drafted sampling between other calls: shapes that change from call to call (its launches are captured once a shape and replayed), other
-searches and training steps on the same handle.  A handle's results are those of a new one."""
+"""Drafted sampling between other calls: shapes that change from call to call (its buffers are kept), other searches and
+training steps on the same handle.  A handle's results are those of a new one."""
 import numpy as np
 import pytest
 
