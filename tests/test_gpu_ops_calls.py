@@ -36,6 +36,11 @@ def test_a_backward_pass_through_a_product_fails(ops, m):
                 z.sum().backward()
         assert gx.grad is None and gb.grad is None
     assert not ops.mx4_linear(x.requires_grad_(), w).detach().requires_grad
+    y = ops.mx4_linear(x, w, bias=bias)                                     # x records a gradient; y may be written in place all the same
+    assert y.requires_grad and not y._is_view()
+    assert torch.equal(y.mul_(2).detach(), 2 * want)
+    with pytest.raises(RuntimeError, match="mx4_linear has no gradient"):
+        y.sum().backward()
 
 
 def test_a_forward_mode_tangent_is_refused(ops):

@@ -47,12 +47,13 @@ def _wrong_place(dev, **tensors):
 
 
 class _NoGradient(torch.autograd.Function):
-    """`y` as it is, on the record of the tensors it was computed from: a backward pass through it fails instead of leaving them out."""
+    """The tensor in `box` as it is, on the record of those it was computed from: a backward pass through it fails instead of leaving them
+    out.  (In a box, since an input that is handed back would be a view, and could not be written in place.)"""
 
     @staticmethod
-    def forward(ctx, y, name, *inputs):
+    def forward(ctx, box, name, *inputs):
         ctx.name = name
-        return y
+        return box[0]
 
     @staticmethod
     def backward(ctx, grad):
@@ -177,7 +178,7 @@ def mx4_matmul(a, w, bias=None, dtype=torch.float32):
     if rc:
         _fail(rc)
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():
-        return _NoGradient.apply(y, "mx4_matmul", bias)
+        return _NoGradient.apply([y], "mx4_matmul", bias)
     return y
 
 
@@ -216,7 +217,7 @@ def mx4_linear(x, w, bias=None):
     if rc:
         _fail(rc)
     if (x.requires_grad or bias is not None and bias.requires_grad) and torch.is_grad_enabled():
-        return _NoGradient.apply(y, "mx4_linear", x, bias)
+        return _NoGradient.apply([y], "mx4_linear", x, bias)
     return y
 
 
