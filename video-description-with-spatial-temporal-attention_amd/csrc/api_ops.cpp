@@ -87,7 +87,7 @@ static int product_ok(const char* who, int64_t m, int64_t n, int64_t k, const vo
     if (!type_ok(dtype)) return refuse(STATTN_EINVAL, "%s: dtype %d is none of STATTN_F32, STATTN_BF16, STATTN_F16", who, dtype);
     if (ld_y < n || ld_y >= (int64_t)1 << 22) return refuse(STATTN_EINVAL, "%s: ld_y (%lld) must be at least n (%lld) and under 2^22", who, (long long)ld_y, (long long)n);
     if (m && n && !y) return refuse(STATTN_EINVAL, "%s: null y", who);
-    // the smallest tile is 64 x 64, so this keeps the workgroups of a launch under 2^22
+    // tiles are 64 x 64 at least, so a launch stays under 2^24 workgroups
     if ((m + 31) / 32 * ((n + 31) / 32) >= (int64_t)1 << 24) return refuse(STATTN_EINVAL, "%s: a product of %lld x %lld is too large for one call", who, (long long)m, (long long)n);
     (void)k;
     return STATTN_OK;
